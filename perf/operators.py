@@ -146,8 +146,8 @@ def _pack(k, v):
     # keys: token, then group g of 8 values of a block, then block: values 32 b + 8 g + 2 p + h in a word's bits 4 p + 16 h
     a = ck.reshape(*lead, 32, nb, 4, 2, 2, 2).permute(*range(n), n, n + 2, n + 1, n + 5, n + 3, n + 4)
     a = (a[..., 0] | (a[..., 1] << 4)).to(torch.uint8).reshape(*lead, -1)
-    # values: eight tokens, then four values, then token: value 4 e + p in a halfword's bits 4 p
-    e = cv.reshape(*lead, 4, 8, d // 4, 2, 2).permute(*range(n), n, n + 2, n + 1, n + 3, n + 4)
+    # values: eight tokens, then 16 i + m, then token: value 64 i + 16 p + m in a halfword's bits 4 p
+    e = cv.reshape(*lead, 4, 8, d // 64, 2, 2, 16).permute(*range(n), n, n + 2, n + 5, n + 1, n + 3, n + 4)
     e = (e[..., 0] | (e[..., 1] << 4)).to(torch.uint8).reshape(*lead, -1)
     by_octet = lambda t: t.reshape(*lead, 4, 8, nb).transpose(-1, -2).contiguous().reshape(*lead, -1).view(torch.uint8)
     return torch.cat([a, e, by_octet(sk), by_octet(sv), lk.contiguous().reshape(*lead, -1).view(torch.uint8), by_octet(lv)], -1)
@@ -160,7 +160,7 @@ def _unpack(rec, d):
     parts = torch.split(rec, [half, half, side, side, side, side], -1)
     nibbles = lambda x: torch.stack([x & 15, x >> 4], -1)
     a = nibbles(parts[0]).reshape(*lead, 32, 4, nb, 2, 2, 2).permute(*range(n), n, n + 2, n + 1, n + 4, n + 5, n + 3)
-    e = nibbles(parts[1]).reshape(*lead, 4, d // 4, 8, 2, 2).permute(*range(n), n, n + 2, n + 1, n + 3, n + 4)
+    e = nibbles(parts[1]).reshape(*lead, 4, d // 64, 16, 8, 2, 2).permute(*range(n), n, n + 3, n + 1, n + 4, n + 5, n + 2)
     ck = a.reshape(*lead, 32, nb, BLOCK).float()
     cv = e.reshape(*lead, 32, nb, BLOCK).float()
     f16 = lambda x: x.contiguous().view(torch.float16).float()
@@ -402,8 +402,9 @@ def _value(st, table, seq, head, slot, which):
         at = t * (d // 2) + (r // 8) * (4 * nb) + 4 * b + bit // 8
         shift = bit % 8
     else:
-        at = 16 * d + (t // 8) * (4 * d) + (j // 4) * 16 + (t % 8) * 2 + (j % 4) // 2
-        shift = 4 * (j % 2)
+        bit = 4 * (j % 64 // 16)
+        at = 16 * d + (t // 8) * (4 * d) + (j // 64 * 16 + j % 16) * 16 + (t % 8) * 2 + bit // 8
+        shift = bit % 8
     code = (flat[rec[..., None] + at].long() >> shift) & 15
     sides = 32 * d
     blocks = torch.arange(nb, device="cuda")
