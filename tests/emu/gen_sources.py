@@ -153,6 +153,36 @@ def build_library(force: bool = False) -> str:
     return LIBRARY
 
 
+# The 4-bit cache: its kernels and C ABI as a library of their own on the model.
+CACHE_FILES = ("homcomp_cache.hpp", "homcomp_cache_kernels.hip", "homcomp_cache_api.hip")
+CACHE_LIBRARY = os.path.join(GEN, "libhomcomp_cache_emu.so")
+CACHE_EDITS = [
+    ('#include "homcomp_cache.hpp"', '#include "cache_emu.hpp"\n#include "homcomp_cache.hpp"\nthread_local emu_operands emu_products;'),
+    ("{ return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x); }", "{ return emu_f32_to_bf16(x); }"),
+]
+
+
+def build_cache_library(force: bool = False) -> str:
+    """The 4-bit cache's entry points and kernels built for the host against the execution model (with the model's allocator)."""
+    import subprocess
+
+    inputs = [os.path.join(CSRC, f) for f in CACHE_FILES] + [os.path.join(INCLUDE, f) for f in ("homcomp.h", "homcomp_cache.h")]
+    inputs += [os.path.join(HERE, f) for f in ("amdgcn_emu.hpp", "cache_emu.hpp", "emu_runtime.hpp", "emu_library.cpp", "gen_sources.py")]
+    if not force and os.path.exists(CACHE_LIBRARY) and all(os.path.getmtime(f) <= os.path.getmtime(CACHE_LIBRARY) for f in inputs):
+        return CACHE_LIBRARY
+    os.makedirs(GEN, exist_ok=True)
+    kernels, api, shared = (open(os.path.join(CSRC, f)).read() for f in ("homcomp_cache_kernels.hip", "homcomp_cache_api.hip", "homcomp_cache.hpp"))
+    kernels = edit(kernels, CACHE_EDITS, "homcomp_cache_kernels.hip")
+    api = edit(api, [('#include "../../include/homcomp_cache.h"', '#include "homcomp_cache.h"')], "homcomp_cache_api.hip")
+    api += "namespace hc { void note_hip_error(int) {} }\n"   # (the library's own is in homcomp_api.hip)
+    for name, text in (("homcomp_cache_kernels.cpp", kernels), ("homcomp_cache_api.cpp", api), ("homcomp_cache.hpp", shared)):
+        open(os.path.join(GEN, name), "w").write(text)
+    subprocess.run([CLANG, *CXXFLAGS, "-O1", "-mf16c", "-mfma", "-ffp-contract=off", "-fPIC", "-shared", "-x", "c++", "-I" + HERE, "-I" + GEN, "-I" + INCLUDE,
+                    "-include", os.path.join(HERE, "emu_library_config.h"), "-o", CACHE_LIBRARY, os.path.join(HERE, "emu_library.cpp"),
+                    os.path.join(GEN, "homcomp_cache_kernels.cpp"), os.path.join(GEN, "homcomp_cache_api.cpp")], check=True)
+    return CACHE_LIBRARY
+
+
 PROGRAMS = ("shim_roundtrip", "ring_allreduce", "homcomp_eval")
 
 

@@ -34,6 +34,19 @@ def load_binding(library_path: str):
     return mod
 
 
+def load_cache_binding(library_path: str):
+    """A second instance of the package's cache binding, bound to `library_path`."""
+    import sys
+    sys.path.insert(0, ROOT) if ROOT not in sys.path else None
+    import __graft_entry__ as entry
+    pkg = entry.load_package()
+    mod = _load(pkg.__name__ + ".cache_on_the_cpu_model", os.path.join(ROOT, "tirocinio-triennale_amd", "cache.py"))
+    library = C.CDLL(library_path)
+    mod._package_lib = lambda: library
+    mod._stream_of = lambda device, stream: 0          # every stream is the synchronous one here
+    return mod
+
+
 class _Host(torch.Tensor):
     """What torch.from_numpy returns here: a CPU tensor over the array whose .cuda() copies it into
     the model's device memory."""

@@ -23,7 +23,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libhomcomp_amd.so")
 RESOURCES = os.path.join(HERE, "kernel_resources.txt")
-SOURCES = ["csrc/homcomp_kernels.hip", "csrc/homcomp_api.hip"]
+SOURCES = ["csrc/homcomp_kernels.hip", "csrc/homcomp_api.hip", "csrc/homcomp_cache_kernels.hip", "csrc/homcomp_cache_api.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -59,6 +59,8 @@ def kernel_label(mangled: str) -> str:
     if name == "k_wave" and t:
         nin, loc, out, pl = (int(v) for v in t.groups())
         return f"k_wave<in={nin},local={_LOCAL.get(loc, loc)},out={_OUT.get(out, out)},planes={_PLANES.get(pl, pl)}>"
+    if name.startswith("k_cache") and (t := re.search(r"I((?:L[ib]\d+E)+)E", mangled)):
+        return name + "<" + ",".join(re.findall(r"L[ib](\d+)E", t.group(1))) + ">"
     t = re.search(r"ILi(\d+)E", mangled)
     return f"{name}<{t.group(1)}>" if t else name
 

@@ -46,6 +46,12 @@ inline bool eb_ok(float eb) { return std::isfinite(eb) && eb > 0.0f; }
 
 }  // namespace
 
+// (for the entry points in other source files, homcomp_cache.hpp)
+namespace hc {
+void note_hip_error(int error);
+void note_hip_error(int error) { g_last_hip_error = error; }
+}  // namespace hc
+
 struct homcomp_workspace {
     int device;
     size_t max_n;
