@@ -159,6 +159,7 @@ CACHE_LIBRARY = os.path.join(GEN, "libhomcomp_cache_emu.so")
 CACHE_EDITS = [
     ('#include "homcomp_cache.hpp"', '#include "cache_emu.hpp"\n#include "homcomp_cache.hpp"\nthread_local emu_operands emu_products;'),
     ("{ return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x); }", "{ return emu_f32_to_bf16(x); }"),
+    ("{ return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }", "{ return emu_f32_to_bf16(a) | (emu_f32_to_bf16(b) << 16); }"),
 ]
 
 

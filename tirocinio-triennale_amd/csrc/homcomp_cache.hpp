@@ -47,7 +47,9 @@ struct AttendArgs {
     int32_t causal, window;     // window 0: none
     float scale;
     float *lse;                 // null: not wanted
-    float *partial;             // of more than one split: per tile and split kColumns * (head_dim + 2) floats
+    float *partial;             // of more than one split: [tile][kColumns][split][head_dim]
+    float *partial_sums;        // [tile][kColumns][split][2]: exponent the part is relative to, sum
+    int32_t columns;            // columns that a tile can have
     const float *prior;
     float *weights;
     uint64_t weight_stride;

@@ -85,8 +85,8 @@ int rows_call(bool store, const homcomp_cache *cache, void *k, void *v, int type
 
 // Shapes of an attention call: column tiles, parts, scratch memory.
 struct AttendPlan {
-    int tiles, splits, split_records;
-    size_t partial_bytes, lse_bytes;
+    int tiles, columns, splits, split_records;
+    size_t partial_bytes, sums_bytes, lse_bytes;
 };
 
 int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, int64_t slots, AttendPlan *p)
@@ -99,22 +99,30 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
     const int group = t->q_heads / c->kv_heads;
     const int64_t most = (int64_t)t->max_length < 0 || (int64_t)t->max_length > slots ? slots : (int64_t)t->max_length;
     p->tiles = (int)(((int64_t)t->max_rows * group + hc::kColumns - 1) / hc::kColumns);
+    p->columns = p->tiles == 1 ? (int)((int64_t)t->max_rows * group) : hc::kColumns;
     int64_t span = most;
     if (t->window && t->window < (size_t)most && (int64_t)(t->window + t->max_rows) < most) span = (int64_t)(t->window + t->max_rows);
     int64_t records = (span + 31) / 32 + 1;   // a window can begin inside a record
     if (records > (most + 31) / 32) records = (most + 31) / 32;
     if (records < 1) records = 1;
     const int64_t units = (int64_t)c->n_seqs * c->kv_heads * p->tiles;
-    // enough workgroups to fill the device, and two records at least for every wave
-    int64_t splits = units ? (4 * kComputeUnits + units - 1) / units : 1;
-    const int64_t fine = (records + 2 * hc::kAttendWaves - 1) / (2 * hc::kAttendWaves);
+    // eight workgroups for every compute unit, so that sequences of different lengths even out, but eight records at least for
+    // every wave (and two where there is little in all)
+    int64_t splits = units ? (8 * kComputeUnits + units - 1) / units : 1;
+    const int64_t least = units * records >= 64 * kComputeUnits ? 8 : 2;
+    const int64_t fine = (records + least * hc::kAttendWaves - 1) / (least * hc::kAttendWaves);
     if (splits > fine) splits = fine;
     int64_t each = (records + splits - 1) / splits;
     each = (each + hc::kAttendWaves - 1) / hc::kAttendWaves * hc::kAttendWaves;
     p->split_records = (int)each;
     p->splits = (int)((records + each - 1) / each);
     if (units * p->splits > kMostWorkgroups || (int64_t)c->n_seqs * c->kv_heads * ((most + 31) / 32) > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
-    if (p->splits > 1) p->partial_bytes = (size_t)units * (size_t)p->splits * hc::kColumns * (size_t)(32 * nb + 2) * sizeof(float);
+    if (units * hc::kColumns > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
+    if (p->splits > 1) {
+        const size_t parts = (size_t)units * (size_t)p->splits * hc::kColumns;
+        p->partial_bytes = parts * (size_t)(32 * nb) * sizeof(float);
+        p->sums_bytes = parts * 2 * sizeof(float);
+    }
     if (t->d_weights && !t->d_lse) p->lse_bytes = (t->n_rows * (size_t)t->q_heads * sizeof(float) + 15) / 16 * 16;
     return HOMCOMP_OK;
 }
@@ -147,7 +155,7 @@ size_t homcomp_cache_attend_scratch(const homcomp_cache *cache, const homcomp_at
     int64_t slots = 0;
     AttendPlan p;
     if (!attention || shape_of(cache, &nb, &slots) || plan_attention(cache, attention, nb, slots, &p)) return 0;
-    return p.partial_bytes + p.lse_bytes;
+    return p.partial_bytes + p.sums_bytes + p.lse_bytes;
 }
 
 int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t, void *stream)
@@ -169,7 +177,7 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t,
         if (!t->d_q || !t->d_out || t->d_q == t->d_out) return HOMCOMP_ERR_INVALID_ARG;
         if (!aligned(t->d_q, bytes_of(t->type)) || !aligned(t->d_out, bytes_of(t->type))) return HOMCOMP_ERR_ALIGNMENT;
     }
-    const size_t need = p.partial_bytes + p.lse_bytes;
+    const size_t need = p.partial_bytes + p.sums_bytes + p.lse_bytes;
     if (need && (!t->d_scratch || t->scratch_bytes < need)) return HOMCOMP_ERR_INVALID_ARG;
     a.q = t->d_q;
     a.out = t->d_out;
@@ -187,8 +195,10 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t,
     a.causal = t->causal ? 1 : 0;
     a.window = t->window > (size_t)kMostSlots ? 0 : (int32_t)t->window;   // (no slot is that far away)
     a.scale = t->scale;
-    a.lse = p.lse_bytes ? (float *)((uint8_t *)t->d_scratch + p.partial_bytes) : t->d_lse;
+    a.lse = p.lse_bytes ? (float *)((uint8_t *)t->d_scratch + p.partial_bytes + p.sums_bytes) : t->d_lse;
     a.partial = (float *)t->d_scratch;
+    a.partial_sums = (float *)((uint8_t *)t->d_scratch + p.partial_bytes);
+    a.columns = p.columns;
     a.prior = t->d_prior;
     a.weights = t->d_weights;
     a.weight_stride = t->weight_stride;

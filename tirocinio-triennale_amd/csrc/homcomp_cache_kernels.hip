@@ -11,6 +11,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 enum : int { kBf16 = 0, kF16 = 1, kF32 = 2 };
@@ -73,6 +74,39 @@ __device__ __forceinline__ void store8(void *base, uint64_t at, const float *x)
         }
     } else {
         for (int i = 0; i < 8; ++i) store_number<TY>(base, at + (uint64_t)i, x[i]);
+    }
+}
+
+// N adjacent numbers (4, 8 or 16) in pieces of 16 bytes where the address allows them, else one by one.
+template <int N, int TY>
+__device__ __forceinline__ void store_run(void *base, uint64_t at, const float *x)
+{
+    constexpr int kSize = TY == kF32 ? 4 : 2;
+    uint8_t *p = (uint8_t *)base + at * kSize;
+    if (N * kSize < 16) {
+        if (((uintptr_t)p & 7u) == 0) {
+            u32x2 w;
+            for (int i = 0; i < 2; ++i) w[i] = TY == kBf16 ? f32_to_bf16(x[2 * i]) | (f32_to_bf16(x[2 * i + 1]) << 16) : f32_to_f16(x[2 * i]) | (f32_to_f16(x[2 * i + 1]) << 16);
+            *(u32x2 *)p = w;
+            return;
+        }
+    } else if (((uintptr_t)p & 15u) == 0) {
+        if (TY == kF32) {
+            for (int i = 0; i < N; i += 4) *(f32x4 *)(p + 4 * i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+        } else {
+            for (int i = 0; i < N; i += 8) store8<TY>(base, at + (uint64_t)i, x + i);
+        }
+        return;
+    }
+    for (int i = 0; i < N; ++i) store_number<TY>(base, at + (uint64_t)i, x[i]);
+}
+// N adjacent 32-bit numbers at a multiple of 16 bytes.
+template <int N>
+__device__ __forceinline__ void load_run(const float *base, uint64_t at, float *x)
+{
+    for (int i = 0; i < N; i += 4) {
+        const f32x4 v = *(const f32x4 *)(base + at + (uint64_t)i);
+        for (int k = 0; k < 4; ++k) x[i + k] = v[k];
     }
 }
 
@@ -279,17 +313,17 @@ constexpr float kNegInf = -INFINITY;
 template <int TY>
 constexpr int query_parts() { return TY == kF32 ? 3 : 1; }
 template <int TY>
-constexpr int weight_parts() { return TY == kF32 ? 3 : (TY == kF16 ? 2 : 1); }
+constexpr int weight_parts() { return TY == kF32 ? 3 : 2; }
 
 template <int NB, int NQ>
 struct Queries {
-    f16x8 q[NB][NQ];    // values 32 b + 8 g .. + 7 of the column's row, scaled; every other pair by 1/16 more
+    f16x8 q[NB][NQ];    // values 32 b + 8 g .. + 7 of the column's row, scaled; where codes stand sixteen times as high by 1/16 more
     bf16x8 sums;        // g-th part (of three) of the sums over each block, times 2^-24
     float factor;       // what turns a score into the exponent of a power of two
     int see_from, see_to;   // slots see_from <= j < see_to are seen
 };
 
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { return f32_to_bf16(a) | (f32_to_bf16(b) << 16); }
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }
 
 // Eight numbers as NP bfloat16 vectors whose sum they are (to 8, 16 or 24 bits).
 template <int NP>
@@ -311,7 +345,7 @@ __device__ __forceinline__ void split_bf16(const float *x, bf16x8 *out)
 }
 
 // column: row * group + head of the group, at or beyond `columns` none (it sees no slot).
-template <int NB, int TY>
+template <int NB, int TY, bool FINE>
 __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int first, int count, int length, int column, int g,
                                              Queries<NB, query_parts<TY>()> &r)
 {
@@ -346,7 +380,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
             for (int i = 0; i < 8; ++i) {
                 const _Float16 part = (_Float16)rest[i];
                 rest[i] -= (float)part;
-                r.q[b][p][i] = (i & 2) ? (_Float16)((float)part * 0.0625f) : part;
+                r.q[b][p][i] = FINE || (i & 2) ? (_Float16)((float)part * 0.0625f) : part;
             }
         }
     }
@@ -360,30 +394,117 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
     r.see_from = a.window > 0 && at + 1 - a.window > 0 ? at + 1 - a.window : 0;
 }
 
-// x[T][r]: the exponent (base 2) of slot 8 g + 4 T + r of the record for the lane's column.
-template <int NB, int NQ>
-__device__ __forceinline__ void record_scores(const uint8_t *rec, int lane, const Queries<NB, NQ> &q, float (&x)[2][4])
+// What a lane holds of a record: rows of the products' operands, and the scales of what it gets back.
+template <int NB>
+struct KeyPart {
+    uint32_t codes[2][NB];      // slots 8 (m / 4) + 4 T + m % 4, m = lane % 16: values 32 b + 8 g .. + 7
+    uint32_t lows[2][NB / 2];   // the same slots' lowest numbers
+    f16x8 steps[NB];            // of slots 8 g .. + 7
+};
+template <int NB>
+struct ValuePart {
+    u32x4 codes[NB / 2];        // slots 8 g .. + 7: values 64 i + 16 p + m
+    f16x8 steps[NB];
+    u32x4 lows;                 // of block m % NB
+    u32x4 own_steps;            // likewise, bits of float16
+};
+// A record on its way: 16-byte pieces lane, lane + 64, .. of it, loaded ahead, then laid into the wave's own part of LDS, from
+// where lanes take what they need (a scale goes to sixteen lanes; LDS hands it to all of them at once).  Keys' codes are laid so that
+// the lanes of a read lie side by side: [half of a row's share][T][g][m] instead of [slot][g][half].
+template <int NB>
+struct RawRecord {
+    static constexpr int kPieces = (80 * NB + 63) / 64;
+    u32x4 piece[kPieces];
+};
+template <int NB>
+__device__ __forceinline__ void load_record(const uint8_t *rec, int lane, RawRecord<NB> &raw)
+{
+    for (int i = 0; i < RawRecord<NB>::kPieces; ++i)
+        if (64 * i + 64 <= 80 * NB || 64 * i + lane < 80 * NB) raw.piece[i] = *(const u32x4 *)(rec + (64 * i + lane) * 16);
+}
+template <int NB>
+__device__ __forceinline__ int key_place(int piece)   // where piece `piece` of the keys' codes is laid
+{
+    if (NB == 2) return piece;
+    constexpr int kHalves = NB / 4;
+    const int half = piece % kHalves, g = piece / kHalves % 4, key = piece / (4 * kHalves);
+    const int T = (key >> 2) & 1, m = 4 * (key >> 3) + (key & 3);
+    return ((half * 2 + T) * 4 + g) * 16 + m;
+}
+template <int NB>
+__device__ __forceinline__ void lay_record(uint8_t *at, int lane, const RawRecord<NB> &raw)
+{
+    for (int i = 0; i < RawRecord<NB>::kPieces; ++i) {
+        const int piece = 64 * i + lane;
+        if (64 * i + 64 <= 80 * NB || piece < 80 * NB) *(u32x4 *)(at + (64 * i < 32 * NB ? key_place<NB>(piece) : piece) * 16) = raw.piece[i];
+    }
+    // a wave's LDS accesses take effect in order; this keeps the compiler from changing it
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// STEPS, LOWS: where the keys' steps and lowest numbers lie, in units of NB bytes.
+template <int NB, uint32_t STEPS = kKeySteps, uint32_t LOWS = kKeyLows>
+__device__ __forceinline__ void take_keys(const uint8_t *at, int lane, KeyPart<NB> &k)
 {
     const int m = lane & 15, g = lane >> 4;
     for (int T = 0; T < 2; ++T) {
         const int key = 8 * (m >> 2) + 4 * T + (m & 3);
-        const uint8_t *codes = rec + key * 16 * NB + g * 4 * NB;
-        const uint8_t *lows = rec + kKeyLows * NB + key * 2 * NB;
-        u32x4 lo = {0, 0, 0, 0};
-        uint32_t w[NB];
-        for (int i = 0; i < NB / 2; ++i) lo[i] = ((const uint32_t *)lows)[i];
-        for (int b = 0; b < NB; ++b) w[b] = ((const uint32_t *)codes)[b];
-        f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), q.sums, f32x4{0, 0, 0, 0}, 0, 0, 0);
-        for (int b = 0; b < NB; ++b) {
-            const uint32_t high = w[b] >> 8;
-            const f16x8 c = __builtin_bit_cast(f16x8, u32x4{w[b] & 0x000f000fu, w[b] & 0x00f000f0u, high & 0x000f000fu, high & 0x00f000f0u});
-            f32x4 part = {0, 0, 0, 0};
-            for (int p = 0; p < NQ; ++p) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, q.q[b][p], part, 0, 0, 0);
-            const f16x4 s = *(const f16x4 *)(rec + kKeySteps * NB + (g * NB + b) * 16 + 8 * T);
-            for (int r = 0; r < 4; ++r) acc[r] = fmaf((float)s[r], part[r], acc[r]);
+        if (NB == 2) {
+            const u32x2 w = *(const u32x2 *)(at + key * 32 + g * 8);
+            k.codes[T][0] = w[0];
+            k.codes[T][1] = w[1];
+        } else {
+            for (int half = 0; half < NB / 4; ++half) {
+                const u32x4 w = *(const u32x4 *)(at + (((half * 2 + T) * 4 + g) * 16 + m) * 16);
+                for (int i = 0; i < 4; ++i) k.codes[T][4 * half + i] = w[i];
+            }
         }
-        for (int r = 0; r < 4; ++r) x[T][r] = acc[r] * q.factor;
+        const uint32_t *lows = (const uint32_t *)(at + LOWS * NB + key * 2 * NB);
+        for (int i = 0; i < NB / 2; ++i) k.lows[T][i] = lows[i];
     }
+    for (int b = 0; b < NB; ++b) k.steps[b] = *(const f16x8 *)(at + STEPS * NB + (g * NB + b) * 16);
+}
+template <int NB>
+__device__ __forceinline__ void take_values(const uint8_t *at, int lane, ValuePart<NB> &v)
+{
+    const int m = lane & 15, g = lane >> 4, own = m & (NB - 1);
+    for (int i = 0; i < NB / 2; ++i) v.codes[i] = *(const u32x4 *)(at + kValueCodes * NB + g * 128 * NB + (i * 16 + m) * 16);
+    for (int b = 0; b < NB; ++b) v.steps[b] = *(const f16x8 *)(at + kValueSteps * NB + (g * NB + b) * 16);
+    v.lows = *(const u32x4 *)(at + kValueLows * NB + (g * NB + own) * 16);
+    v.own_steps = *(const u32x4 *)(at + kValueSteps * NB + (g * NB + own) * 16);
+}
+
+// The four pairs of codes of a word, as numbers of 16 bits below or at the foot of the normal range.  FINE: all at bits 4 .. 7, for two
+// more shifts: the matrix unit aligns products by their exponents, a number below the normal range counts as if it
+// had the smallest one, and what a product has in front of its first bit it lacks behind the last (measured for a score of a few
+// units: 4e-6 off with codes at bits 0 .. 3, 3e-7 at bits 4 .. 7).
+template <bool FINE>
+__device__ __forceinline__ u32x4 code_pairs(uint32_t w)
+{
+    if (FINE) return u32x4{(w << 4) & 0x00f000f0u, w & 0x00f000f0u, (w >> 4) & 0x00f000f0u, (w >> 8) & 0x00f000f0u};
+    const uint32_t high = w >> 8;
+    return u32x4{w & 0x000f000fu, w & 0x00f000f0u, high & 0x000f000fu, high & 0x00f000f0u};
+}
+
+// x[T][r]: the score, short of `factor`, of slot 8 g + 4 T + r of the record for the lane's column.
+template <int NB, int NQ, bool FINE>
+__device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Queries<NB, NQ> &q, f32x4 (&x)[2])
+{
+    f32x4 part[2][NB];
+    for (int T = 0; T < 2; ++T) {
+        u32x4 lo = {0, 0, 0, 0};
+        for (int i = 0; i < NB / 2; ++i) lo[i] = k.lows[T][i];
+        x[T] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), q.sums, f32x4{0, 0, 0, 0}, 0, 0, 0);
+        for (int b = 0; b < NB; ++b) {
+            const f16x8 c = __builtin_bit_cast(f16x8, code_pairs<FINE>(k.codes[T][b]));
+            part[T][b] = f32x4{0, 0, 0, 0};
+            for (int p = 0; p < NQ; ++p) part[T][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, q.q[b][p], part[T][b], 0, 0, 0);
+        }
+    }
+    for (int T = 0; T < 2; ++T)
+        for (int b = 0; b < NB; ++b)
+            for (int r = 0; r < 4; ++r) x[T][r] = fmaf((float)k.steps[b][4 * T + r], part[T][b][r], x[T][r]);
 }
 
 // Records that a tile's columns can see at all: [*from, *to).
@@ -399,6 +520,15 @@ __device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int
     *from = begin >> 5;
     *to = begin < end ? (end + 31) >> 5 : begin >> 5;
 }
+// Slots that every one of a tile's columns sees: [*from, *to).
+__device__ __forceinline__ void seen_by_all(const AttendArgs &a, int count, int length, int tile, int *from, int *to)
+{
+    const int first_row = tile * kColumns / a.group;
+    int last_row = (tile * kColumns + kColumns - 1) / a.group;
+    if (last_row >= count) last_row = count - 1;
+    *to = a.causal && length - count + first_row + 1 < length ? length - count + first_row + 1 : length;
+    *from = a.window > 0 && length - count + last_row + 1 - a.window > 0 ? length - count + last_row + 1 - a.window : 0;
+}
 
 // One column's share of a workgroup's result: out rows of 16 columns, 16 threads each.
 template <int NB, int TY>
@@ -410,20 +540,120 @@ __device__ __forceinline__ void write_result(const AttendArgs &a, int h, int fir
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     for (int i = 0; i < N; ++i) x[i] = total == 0.0f ? 0.0f : o[i] * inv;
     const uint64_t at = (uint64_t)(first + row) * a.out_row_stride + (uint64_t)(h * a.group + head) * a.out_head_stride + (uint64_t)(part * N);
-    for (int i = 0; i < N; ++i) store_number<TY>(a.out, at + (uint64_t)i, x[i]);
+    store_run<N, TY>(a.out, at, x);
     if (a.lse && part == 0)
         a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)] =
             total == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-template <int NB, int TY>
-__global__ __launch_bounds__(256) void k_cache_attend(AttendArgs a)
+// What a wave has gathered for its columns.
+template <int NB>
+struct Gathered {
+    f32x4 o[NB / 2][4];   // sum of (code - 8 or 7) * p s_b, values 64 i + 16 p + 4 g + r, times 2^-69 (2^-65 where codes stand higher)
+    f32x4 low;            // what block 4 g + r adds to all its values, times 2^64
+    float top;            // exponent p is relative to; at most 8 below the largest so far
+    float total;          // sum of the lane's p, times 2^64
+};
+
+// One record.  A new reference exponent costs a multiplication of everything gathered, so it is taken only where a weight
+// would exceed 2^8 (32-bit sums have room for that); a lane looks at its own eight slots alone, and lanes exchange only then.
+template <int NB, int NQ, int NP, bool FINE, bool MASKED>
+__device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<NB, NQ> &q, int lane, int slot0, int length, Gathered<NB> &s)
+{
+    f32x4 x[2];
+    KeyPart<NB> k;
+    take_keys<NB>(at, lane, k);
+    record_scores<NB, NQ, FINE>(k, q, x);
+    ValuePart<NB> v;
+    take_values<NB>(at, lane, v);
+    // 2^64 goes in with the exponent, except for 32-bit results: next to 64 an exponent keeps 2^-19, too little for them
+    constexpr float kUp = NP == 3 ? 0.0f : 64.0f;
+    float e[8];
+    bool seen[8];
+    const float bias = kUp - s.top;      // (nothing seen yet: +infinity, which asks for a reference)
+    float most = kNegInf;
+    for (int i = 0; i < 8; ++i) {
+        seen[i] = !MASKED || (slot0 + i >= q.see_from && slot0 + i < q.see_to);
+        e[i] = seen[i] ? fmaf(x[i >> 2][i & 3], q.factor, bias) : kNegInf;
+        most = fmaxf(most, e[i]);
+    }
+    if (__builtin_amdgcn_ballot_w64(most > kUp + 8.0f) != 0) {
+        most = kNegInf;
+        for (int i = 0; i < 8; ++i)
+            if (seen[i]) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const float now = fmaxf(s.top, most);
+        const float shrink = now == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(s.top - now);   // (nothing so far: 0)
+        s.top = now;
+        s.total *= shrink;
+        for (int r = 0; r < 4; ++r) {
+            s.low[r] *= shrink;
+            for (int i = 0; i < NB / 2; ++i)
+                for (int n = 0; n < 4; ++n) s.o[i][n][r] *= shrink;
+        }
+        for (int i = 0; i < 8; ++i) e[i] = seen[i] ? fmaf(x[i >> 2][i & 3], q.factor, kUp - now) : kNegInf;
+    }
+    float p[8];
+    for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(e[i]);
+        if (NP == 3) p[i] *= 0x1p64f;
+        s.total += p[i];
+    }
+    // Codes count from the middle, c - 8 in even slots and c - 7 in odd ones (numbers of the codes' own form; on the average the
+    // middle itself), the rest is lo + 8 s or lo + 7 s: with codes from 0 the two sums would grow with the number of slots and nearly
+    // cancel where a block's values lie around zero, each with roundings of its own.
+    u32x4 middle[NP];
+    {
+        float mid[8];
+        for (int i = 0; i < 8; ++i) {
+            const float step = (float)__builtin_bit_cast(f16x8, v.own_steps)[i];
+            mid[i] = fmaf(step, (i & 1) ? 7.0f : 8.0f, (i & 1) ? __builtin_bit_cast(float, v.lows[i >> 1] & 0xffff0000u) : bf16_to_f32(v.lows[i >> 1]));
+            // a slot that only some columns see, or none: a NaN there reaches those that see it by p s_b
+            if (MASKED && (slot0 + i >= length || !(step == step))) mid[i] = 0.0f;
+        }
+        bf16x8 parts[NP];
+        split_bf16<NP>(mid, parts);
+        for (int n = 0; n < NP; ++n) middle[n] = __builtin_bit_cast(u32x4, parts[n]);
+    }
+    bf16x8 w[NP];
+    split_bf16<NP>(p, w);
+    for (int n = 0; n < NP; ++n)
+        for (int e2 = 0; n + e2 < NP; ++e2)
+            s.low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, middle[n]), w[e2], s.low, 0, 0, 0);
+    for (int b = 0; b < NB; ++b) {
+        float ps[8];
+        for (int i = 0; i < 8; ++i) ps[i] = seen[i] ? fmaf((float)v.steps[b][i], p[i], 0.0f) : 0.0f;
+        split_bf16<NP>(ps, w);
+        const u32x4 codes = v.codes[b >> 1];
+        constexpr bool kFineValues = NP == 3;
+        for (int n = 0; n < 2; ++n) {
+            u32x4 c;
+            for (int i = 0; i < 4; ++i) c[i] = code_pairs<kFineValues>(codes[i])[2 * (b & 1) + n];
+            const uint32_t back = kFineValues || n ? 0x80708080u : 0x80078008u;
+            f32x4 &o = s.o[b >> 1][2 * (b & 1) + n];
+            for (int e2 = 0; e2 < NP; ++e2) {
+                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), w[e2], o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{back, back, back, back}), w[e2], o, 0, 0, 0);
+            }
+        }
+    }
+}
+
+template <int NB, int TY, bool FINE>
+__global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) void k_cache_attend(AttendArgs a)
 {
     constexpr int NQ = query_parts<TY>(), NP = weight_parts<TY>(), D = 32 * NB;
-    __shared__ float s_o[kAttendWaves][kColumns][D + 4];
+    // the waves' records on their way, and afterwards their results
+    constexpr int kMem = kAttendWaves * (kColumns * (D + 4) * 4 > (int)record_bytes(NB) ? kColumns * (D + 4) * 4 : (int)record_bytes(NB));
+    __shared__ __align__(16) uint8_t s_mem[kMem];
+    float (*s_o)[kColumns][D + 4] = (float (*)[kColumns][D + 4])s_mem;
     __shared__ float s_top[kAttendWaves][kColumns], s_total[kAttendWaves][kColumns];
-    const int split = (int)(blockIdx.x % (unsigned)a.splits);
-    const uint32_t unit = blockIdx.x / (unsigned)a.splits;    // (sequence, head, tile)
+    // parts outermost: workgroups go to the eight dies in turn, and later parts are the ones that shorter sequences lack (parts
+    // innermost: half of the compute units idle on a batch of lengths from a tenth to all of 8192, 144 us instead of 92)
+    const uint32_t units = gridDim.x / (unsigned)a.splits;
+    const int split = (int)(blockIdx.x / units);
+    const uint32_t unit = blockIdx.x % units;    // (sequence, head, tile)
     const int tile = (int)(unit % (unsigned)a.tiles);
     const int h = (int)(unit / (unsigned)a.tiles % (unsigned)a.c.kv_heads);
     const int s = (int)(unit / (unsigned)a.tiles / (unsigned)a.c.kv_heads);
@@ -432,71 +662,44 @@ __global__ __launch_bounds__(256) void k_cache_attend(AttendArgs a)
     const int length = sequence_length(a.c, s);
     if (count > a.max_rows) count = a.max_rows;
     if (tile * kColumns >= count * a.group) return;
-    int from, to;
+    int from, to, all_from, all_to;
     seen_records(a, count, length, tile, &from, &to);
+    seen_by_all(a, count, length, tile, &all_from, &all_to);
     from += split * a.split_records;
     if (split > 0 && from >= to) return;
     if (to > from + a.split_records) to = from + a.split_records;
 
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     Queries<NB, NQ> q;
-    load_queries<NB, TY>(a, h, first, count, length, tile * kColumns + n, g, q);
-    f32x4 o[NB / 2][4], low = {0, 0, 0, 0};
+    load_queries<NB, TY, FINE>(a, h, first, count, length, tile * kColumns + n, g, q);
+    Gathered<NB> acc;
+    acc.low = f32x4{0, 0, 0, 0};
     for (int i = 0; i < NB / 2; ++i)
-        for (int p = 0; p < 4; ++p) o[i][p] = f32x4{0, 0, 0, 0};
-    float top = kNegInf, total = 0.0f;
-
-    for (int it = from + wave; it < to; it += kAttendWaves) {
-        const uint8_t *rec = record_of(a.c, a.c.table, a.c.table_stride, s, h, it * kRecordSlots, NB);
-        if (!rec) continue;
-        float x[2][4];
-        record_scores<NB, NQ>(rec, lane, q, x);
-        const int slot0 = it * kRecordSlots + 8 * g;
-        bool seen[8];
-        float most = kNegInf;
-        for (int i = 0; i < 8; ++i) {
-            seen[i] = slot0 + i >= q.see_from && slot0 + i < q.see_to;
-            if (seen[i]) most = fmaxf(most, x[i >> 2][i & 3]);
+        for (int p = 0; p < 4; ++p) acc.o[i][p] = f32x4{0, 0, 0, 0};
+    acc.top = kNegInf;
+    acc.total = 0.0f;
+    uint8_t *stage = s_mem + wave * (int)record_bytes(NB);
+    RawRecord<NB> raw;
+    int it = from + wave;
+    const uint8_t *rec = it < to ? record_of(a.c, a.c.table, a.c.table_stride, s, h, it * kRecordSlots, NB) : nullptr;
+    if (rec) load_record<NB>(rec, lane, raw);
+    while (it < to) {
+        const int next = it + kAttendWaves;
+        const uint8_t *next_rec = next < to ? record_of(a.c, a.c.table, a.c.table_stride, s, h, next * kRecordSlots, NB) : nullptr;
+        if (rec) lay_record<NB>(stage, lane, raw);
+        if (next_rec) load_record<NB>(next_rec, lane, raw);
+        if (rec) {
+            if (it * kRecordSlots >= all_from && (it + 1) * kRecordSlots <= all_to)
+                attend_record<NB, NQ, NP, FINE, false>(stage, q, lane, it * kRecordSlots + 8 * g, length, acc);
+            else
+                attend_record<NB, NQ, NP, FINE, true>(stage, q, lane, it * kRecordSlots + 8 * g, length, acc);
         }
-        most = fmaxf(most, __shfl_xor(most, 16, 64));
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const float now = fmaxf(top, most), ref = now == kNegInf ? 0.0f : now;
-        const float shrink = __builtin_amdgcn_exp2f(top - ref);   // (nothing so far: 0)
-        top = now;
-        float p[8];
-        total *= shrink;
-        for (int i = 0; i < 8; ++i) {
-            p[i] = seen[i] ? __builtin_amdgcn_exp2f(x[i >> 2][i & 3] - ref + 64.0f) : 0.0f;
-            total += p[i];
-        }
-        for (int r = 0; r < 4; ++r) {
-            low[r] *= shrink;
-            for (int i = 0; i < NB / 2; ++i)
-                for (int k = 0; k < 4; ++k) o[i][k][r] *= shrink;
-        }
-        // what the values' lowest numbers contribute; slots behind the last one may hold anything
-        u32x4 lows = *(const u32x4 *)(rec + kValueLows * NB + (g * NB + (n < NB ? n : NB - 1)) * 16);
-        for (int i = 0; i < 4; ++i) {
-            if (slot0 + 2 * i >= length) lows[i] &= 0xffff0000u;
-            if (slot0 + 2 * i + 1 >= length) lows[i] &= 0x0000ffffu;
-        }
-        bf16x8 w[NP];
-        split_bf16<NP>(p, w);
-        for (int k = 0; k < NP; ++k) low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lows), w[k], low, 0, 0, 0);
-        for (int b = 0; b < NB; ++b) {
-            const f16x8 step = *(const f16x8 *)(rec + kValueSteps * NB + (g * NB + b) * 16);
-            float ps[8];
-            for (int i = 0; i < 8; ++i) ps[i] = seen[i] ? p[i] * (float)step[i] : 0.0f;
-            split_bf16<NP>(ps, w);
-            const u32x4 codes = *(const u32x4 *)(rec + kValueCodes * NB + g * 128 * NB + ((b >> 1) * 16 + n) * 16);
-            for (int k = 0; k < 2; ++k) {
-                u32x4 c;
-                for (int i = 0; i < 4; ++i) c[i] = ((b & 1) ? codes[i] >> 8 : codes[i]) & (k ? 0x00f000f0u : 0x000f000fu);
-                for (int e = 0; e < NP; ++e)
-                    o[b >> 1][2 * (b & 1) + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), w[e], o[b >> 1][2 * (b & 1) + k], 0, 0, 0);
-            }
-        }
+        it = next;
+        rec = next_rec;
     }
+    __syncthreads();
+    float total = acc.total;
+    const float top = acc.top;
 
     // the waves' results meet in LDS
     total += __shfl_xor(total, 16, 64);
@@ -509,12 +712,8 @@ __global__ __launch_bounds__(256) void k_cache_attend(AttendArgs a)
         for (int p = 0; p < 4; ++p) {
             const int b = 2 * i + (p >> 1);
             f32x4 v;
-            float base = 0.0f;
-            for (int r = 0; r < 4; ++r) {
-                const float other = __shfl(low[r], n + 16 * (b >> 2), 64);
-                if (r == (b & 3)) base = other * 0x1p-64f;
-            }
-            for (int r = 0; r < 4; ++r) v[r] = fmaf(o[i][p][r], (p & 1) ? 0x1p65f : 0x1p69f, base);
+            const float base = __shfl(acc.low[b & 3], n + 16 * (b >> 2), 64) * 0x1p-64f;
+            for (int r = 0; r < 4; ++r) v[r] = fmaf(acc.o[i][p][r], NP == 3 || (p & 1) ? 0x1p65f : 0x1p69f, base);
             *(f32x4 *)&s_o[wave][n][64 * i + 16 * p + 4 * g] = v;
         }
     }
@@ -530,94 +729,178 @@ __global__ __launch_bounds__(256) void k_cache_attend(AttendArgs a)
         sum = fmaf(s_total[w][column], f, sum);
         for (int i = 0; i < 2 * NB; ++i) x[i] = fmaf(s_o[w][column][part * 2 * NB + i], f, x[i]);
     }
+    if (tile * kColumns + column >= count * a.group) return;
     if (a.splits > 1) {
-        float *to_part = a.partial + (uint64_t)blockIdx.x * (kColumns * (D + 2));
-        for (int i = 0; i < 2 * NB; ++i) to_part[column * D + part * 2 * NB + i] = x[i];
+        const uint64_t at = ((uint64_t)unit * kColumns + (uint32_t)column) * (uint32_t)a.splits + (uint32_t)split;
+        store_run<2 * NB, kF32>(a.partial, at * D + (uint32_t)(part * 2 * NB), x);
         if (part == 0) {
-            to_part[kColumns * D + column] = all;
-            to_part[kColumns * D + kColumns + column] = sum;
+            a.partial_sums[2 * at] = all;
+            a.partial_sums[2 * at + 1] = sum;
         }
-    } else if (tile * kColumns + column < count * a.group) {
+    } else {
         write_result<NB, TY>(a, h, first, tile * kColumns + column, part, all, sum, x);
     }
 }
 
-// Joins the parts of a tile.
+// Joins the parts of a column: a workgroup each, its waves taking parts in turn, 2 NB of the column's values a lane (the waves' other
+// lanes further parts).
 template <int NB, int TY>
 __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
 {
-    constexpr int D = 32 * NB;
-    const int tile = (int)(blockIdx.x % (unsigned)a.tiles);
-    const int h = (int)(blockIdx.x / (unsigned)a.tiles % (unsigned)a.c.kv_heads);
-    const int s = (int)(blockIdx.x / (unsigned)a.tiles / (unsigned)a.c.kv_heads);
+    constexpr int D = 32 * NB, kStrands = 16;   // 16 lanes hold a column
+    __shared__ float s_sum[kStrands][D + 4];
+    __shared__ float s_total[kStrands], s_top[kStrands];
+    const int column = (int)(blockIdx.x % (unsigned)a.columns);
+    const uint32_t unit = blockIdx.x / (unsigned)a.columns;
+    const int tile = (int)(unit % (unsigned)a.tiles);
+    const int h = (int)(unit / (unsigned)a.tiles % (unsigned)a.c.kv_heads);
+    const int s = (int)(unit / (unsigned)a.tiles / (unsigned)a.c.kv_heads);
     int first, count;
     rows_of(a.starts, s, a.n_rows, &first, &count);
     const int length = sequence_length(a.c, s);
     if (count > a.max_rows) count = a.max_rows;
-    const int column = threadIdx.x >> 4, part = threadIdx.x & 15;
     if (tile * kColumns + column >= count * a.group) return;
     int from, to;
     seen_records(a, count, length, tile, &from, &to);
     int parts = (to - from + a.split_records - 1) / a.split_records;
     if (parts < 1) parts = 1;
     if (parts > a.splits) parts = a.splits;
-    const float *at = a.partial + (uint64_t)blockIdx.x * (uint64_t)a.splits * (kColumns * (D + 2));
-    float all = kNegInf;
-    for (int i = 0; i < parts; ++i) all = fmaxf(all, at[(uint64_t)i * (kColumns * (D + 2)) + kColumns * D + column]);
-    float sum = 0.0f, x[2 * NB];
+    const uint64_t at = ((uint64_t)unit * kColumns + (uint32_t)column) * (uint32_t)a.splits;
+    const int strand = threadIdx.x >> 4, place = threadIdx.x & 15;
+    float x[2 * NB], total = 0.0f, top = kNegInf;
     for (int i = 0; i < 2 * NB; ++i) x[i] = 0.0f;
-    for (int k = 0; k < parts; ++k) {
-        const float *p = at + (uint64_t)k * (kColumns * (D + 2));
-        const float f = all == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(p[kColumns * D + column] - all);
-        sum = fmaf(p[kColumns * D + kColumns + column], f, sum);
-        for (int i = 0; i < 2 * NB; ++i) x[i] = fmaf(p[column * D + part * 2 * NB + i], f, x[i]);
+    for (int k = strand; k < parts; k += kStrands) top = fmaxf(top, a.partial_sums[2 * (at + (uint32_t)k)]);
+    if (place == 0) s_top[strand] = top;
+    __syncthreads();
+    for (int k = 0; k < kStrands; ++k) top = fmaxf(top, s_top[k]);
+    for (int k = strand; k < parts; k += kStrands) {
+        const uint64_t p = at + (uint32_t)k;
+        const float f = top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(a.partial_sums[2 * p] - top);
+        float y[2 * NB];
+        load_run<2 * NB>(a.partial, p * D + (uint32_t)(place * 2 * NB), y);
+        total = fmaf(a.partial_sums[2 * p + 1], f, total);
+        for (int i = 0; i < 2 * NB; ++i) x[i] = fmaf(y[i], f, x[i]);
     }
-    write_result<NB, TY>(a, h, first, tile * kColumns + column, part, all, sum, x);
+    for (int i = 0; i < 2 * NB; ++i) s_sum[strand][place * 2 * NB + i] = x[i];
+    if (place == 0) s_total[strand] = total;
+    __syncthreads();
+    if (strand != 0) return;
+    const int strands = parts < kStrands ? parts : kStrands;
+    for (int k = 1; k < strands; ++k) {
+        total += s_total[k];
+        for (int i = 0; i < 2 * NB; ++i) x[i] += s_sum[k][place * 2 * NB + i];
+    }
+    write_result<NB, TY>(a, h, first, tile * kColumns + column, place, top, total, x);
 }
 
-// The attention each slot received: a wave takes a record and goes over all columns of its sequence and head, computing the scores
-// again (a pass over the keys costs less than keeping a score for every column and slot), and adds in the columns' order.
+// The attention each slot received.  A wave holds kHeldRecords records' keys in LDS and goes over all columns of their sequence and head,
+// computing the scores again, and adds in the columns' order.  (Keeping the scores of the attention kernel instead would write and
+// read 4 bytes for every column and slot: with four columns 32 bytes a slot, with eight 64, against the 80 of the keys of 128 values.)
+constexpr int kHeldRecords = 4;
+
+// The keys of a record: codes, steps, lowest numbers, in 16-byte pieces lane, lane + 64, ..
+template <int NB>
+struct RawKeys {
+    static constexpr int kPieces = (40 * NB + 63) / 64;
+    u32x4 piece[kPieces];
+};
+template <int NB>
+__device__ __forceinline__ void load_raw_keys(const uint8_t *rec, int lane, RawKeys<NB> &raw)
+{
+    for (int i = 0; i < RawKeys<NB>::kPieces; ++i) {
+        const int u = 64 * i + lane;
+        if (u < 40 * NB) raw.piece[i] = *(const u32x4 *)(rec + (u < 32 * NB ? u : (u < 36 * NB ? u + 32 * NB : u + 36 * NB)) * 16);
+    }
+}
+template <int NB>
+__device__ __forceinline__ void lay_keys(uint8_t *at, int lane, const RawKeys<NB> &raw)
+{
+    for (int i = 0; i < RawKeys<NB>::kPieces; ++i) {
+        const int u = 64 * i + lane;
+        if (u < 40 * NB) *(u32x4 *)(at + (u < 32 * NB ? key_place<NB>(u) : u) * 16) = raw.piece[i];
+    }
+}
+
+// v[i] summed over the sixteen lanes of a row: lane n gets that of i = 4 (n & 1) + (n & 2) + (n >> 2 & 1).
+__device__ __forceinline__ float sum_over_row(const float *v, int n)
+{
+    float a[4], b[2];
+    for (int i = 0; i < 4; ++i) {
+        const float give = (n & 1) ? v[i] : v[4 + i], keep = (n & 1) ? v[4 + i] : v[i];
+        a[i] = keep + __shfl_xor(give, 1, 64);
+    }
+    for (int i = 0; i < 2; ++i) {
+        const float give = (n & 2) ? a[i] : a[2 + i], keep = (n & 2) ? a[2 + i] : a[i];
+        b[i] = keep + __shfl_xor(give, 2, 64);
+    }
+    const float give = (n & 4) ? b[0] : b[1], keep = (n & 4) ? b[1] : b[0];
+    const float c = keep + __shfl_xor(give, 4, 64);
+    return c + __shfl_xor(c, 8, 64);
+}
+
 template <int NB, int TY>
 __global__ __launch_bounds__(256) void k_cache_weights(AttendArgs a, int records)
 {
-    constexpr int NQ = query_parts<TY>();
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const uint32_t groups = ((uint32_t)records + kAttendWaves - 1) / kAttendWaves;
-    const int it = (int)(blockIdx.x % groups) * kAttendWaves + wave;
+    constexpr int NQ = query_parts<TY>(), kBytes = 640 * NB;
+    __shared__ __align__(16) uint8_t s_mem[kAttendWaves][kHeldRecords][kBytes];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const uint32_t groups = ((uint32_t)records + kAttendWaves * kHeldRecords - 1) / (kAttendWaves * kHeldRecords);
+    const int it0 = (int)(blockIdx.x % groups) * (kAttendWaves * kHeldRecords) + wave * kHeldRecords;
     const int h = (int)(blockIdx.x / groups % (unsigned)a.c.kv_heads);
     const int s = (int)(blockIdx.x / groups / (unsigned)a.c.kv_heads);
     int first, count;
     rows_of(a.starts, s, a.n_rows, &first, &count);
     const int length = sequence_length(a.c, s);
     if (count > a.max_rows) count = a.max_rows;
-    if (it * kRecordSlots >= length) return;
-    const uint8_t *rec = record_of(a.c, a.c.table, a.c.table_stride, s, h, it * kRecordSlots, NB);
-    float sum[8];
-    for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
-    const int slot0 = it * kRecordSlots + 8 * g;
+    if (it0 * kRecordSlots >= length) return;
+    bool there[kHeldRecords];
+    RawKeys<NB> raw[kHeldRecords];
+    for (int k = 0; k < kHeldRecords; ++k) {
+        const uint8_t *rec = (it0 + k) * kRecordSlots < length ? record_of(a.c, a.c.table, a.c.table_stride, s, h, (it0 + k) * kRecordSlots, NB) : nullptr;
+        there[k] = rec != nullptr;
+        if (rec) load_raw_keys<NB>(rec, lane, raw[k]);
+    }
+    for (int k = 0; k < kHeldRecords; ++k)
+        if (there[k]) lay_keys<NB>(s_mem[wave][k], lane, raw[k]);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    float sum[kHeldRecords][8];
+    for (int k = 0; k < kHeldRecords; ++k)
+        for (int i = 0; i < 8; ++i) sum[k][i] = 0.0f;
     for (int tile = 0; tile * kColumns < count * a.group; ++tile) {
         int from, to;
         seen_records(a, count, length, tile, &from, &to);
-        if (!rec || it < from || it >= to) continue;
+        if (it0 + kHeldRecords <= from || it0 >= to) continue;
         const int column = tile * kColumns + n;
         Queries<NB, NQ> q;
-        load_queries<NB, TY>(a, h, first, count, length, column, g, q);
+        load_queries<NB, TY, true>(a, h, first, count, length, column, g, q);
         float lse = 0.0f;
         if (column < count * a.group) {
             const int row = column / a.group, head = column - row * a.group;
             lse = a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)];
         }
-        float x[2][4];
-        record_scores<NB, NQ>(rec, lane, q, x);
-        for (int i = 0; i < 8; ++i)
-            if (slot0 + i >= q.see_from && slot0 + i < q.see_to) sum[i] += __builtin_amdgcn_exp2f(fmaf(lse, -kLog2e, x[i >> 2][i & 3]));
+        for (int k = 0; k < kHeldRecords; ++k) {
+            if (!there[k]) continue;
+            KeyPart<NB> keys;
+            take_keys<NB, 512, 576>(s_mem[wave][k], lane, keys);
+            f32x4 x[2];
+            record_scores<NB, NQ, true>(keys, q, x);
+            const int slot0 = (it0 + k) * kRecordSlots + 8 * g;
+            for (int i = 0; i < 8; ++i)
+                if (slot0 + i >= q.see_from && slot0 + i < q.see_to)
+                    sum[k][i] += __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, lse * -kLog2e));
+        }
     }
-    for (int i = 0; i < 8; ++i)
-        for (int d = 1; d < 16; d <<= 1) sum[i] += __shfl_xor(sum[i], d, 64);
-    if (n != 0) return;
-    const uint64_t at = ((uint64_t)s * a.c.kv_heads + h) * a.weight_stride + (uint64_t)slot0;
-    for (int i = 0; i < 8; ++i)
-        if (slot0 + i < length) a.weights[at + i] = (a.prior ? a.prior[at + i] : 0.0f) + sum[i];
+    const int i = 4 * (n & 1) + (n & 2) + ((n >> 2) & 1);
+    for (int k = 0; k < kHeldRecords; ++k) {
+        const float all = sum_over_row(sum[k], n);
+        const int slot = (it0 + k) * kRecordSlots + 8 * g + i;
+        if (n < 8 && slot < length) {
+            const uint64_t at = ((uint64_t)s * a.c.kv_heads + h) * a.weight_stride + (uint64_t)slot;
+            a.weights[at] = (a.prior ? a.prior[at] : 0.0f) + all;
+        }
+    }
 }
 
 // ---------------------------------------------------------------- eviction
@@ -722,7 +1005,7 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
 template <int NB>
 __global__ __launch_bounds__(256) void k_cache_move(EvictArgs a, int records)
 {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const uint32_t groups = ((uint32_t)records + 3) / 4;
     const int it = (int)(blockIdx.x % groups) * 4 + wave;
     const int h = (int)(blockIdx.x / groups % (unsigned)a.c.kv_heads);
@@ -793,15 +1076,21 @@ template <int NB, int TY>
 static hipError_t attend_of(const AttendArgs &a, hipStream_t s)
 {
     const uint32_t tiles = (uint32_t)a.c.n_seqs * (uint32_t)a.c.kv_heads * (uint32_t)a.tiles;
-    hipLaunchKernelGGL((k_cache_attend<NB, TY>), dim3(tiles * (uint32_t)a.splits), dim3(256), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && a.splits > 1) {
-        hipLaunchKernelGGL((k_cache_join<NB, TY>), dim3(tiles), dim3(256), 0, s, a);
+    hipError_t e = hipSuccess;
+    if (tiles) {
+        // where weights are wanted the sums have to be those of the scores that they are taken from
+        const dim3 grid(tiles * (uint32_t)a.splits);
+        if (TY == kF32 || a.weights) hipLaunchKernelGGL((k_cache_attend<NB, TY, true>), grid, dim3(256), 0, s, a);
+        else if constexpr (TY != kF32) hipLaunchKernelGGL((k_cache_attend<NB, TY, false>), grid, dim3(256), 0, s, a);
         e = hipGetLastError();
+        if (e == hipSuccess && a.splits > 1) {
+            hipLaunchKernelGGL((k_cache_join<NB, TY>), dim3(tiles * (uint32_t)a.columns), dim3(256), 0, s, a);
+            e = hipGetLastError();
+        }
     }
     if (e == hipSuccess && a.weights) {
         const uint32_t records = ((uint32_t)a.c.max_slots + kRecordSlots - 1) / kRecordSlots;
-        const uint32_t groups = (records + kAttendWaves - 1) / kAttendWaves;
+        const uint32_t groups = (records + kAttendWaves * kHeldRecords - 1) / (kAttendWaves * kHeldRecords);
         hipLaunchKernelGGL((k_cache_weights<NB, TY>), dim3(groups * (uint32_t)a.c.kv_heads * (uint32_t)a.c.n_seqs), dim3(256), 0, s, a, (int)records);
         e = hipGetLastError();
     }
