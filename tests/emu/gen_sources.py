@@ -58,9 +58,9 @@ LAUNCHERS = "// ----------------------------------------------------------------
 
 
 def edit(text: str, edits, what: str) -> str:
-    for old, new in edits:
-        if text.count(old) != 1:
-            raise SystemExit(f"gen_sources: expected exactly one occurrence in {what} of: {old!r}")
+    for old, new, *count in edits:
+        if text.count(old) != (count[0] if count else 1):
+            raise SystemExit(f"gen_sources: expected {count[0] if count else 'exactly one'} occurrence(s) in {what} of: {old!r}")
         text = text.replace(old, new)
     for space in ("__attribute__((address_space(3))) ", "__attribute__((address_space(1))) "):
         text = text.replace(space, "")
@@ -159,6 +159,10 @@ CACHE_LIBRARY = os.path.join(GEN, "libhomcomp_cache_emu.so")
 CACHE_EDITS = [
     ('#include "homcomp_cache.hpp"', '#include "cache_emu.hpp"\n#include "homcomp_cache.hpp"\nthread_local emu_operands emu_products;'),
     ("{ return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x); }", "{ return emu_f32_to_bf16(x); }"),
+    ('asm volatile("" : "+v"(zero));', "", 2),
+    ('asm volatile("" : "+v"(from));', "", 3),
+    ("{ return __builtin_elementwise_fma(a, b, c); }",
+     "{ return f16x2{(_Float16)fmaf((float)a[0], (float)b[0], (float)c[0]), (_Float16)fmaf((float)a[1], (float)b[1], (float)c[1])}; }"),
     ("{ return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }", "{ return emu_f32_to_bf16(a) | (emu_f32_to_bf16(b) << 16); }"),
 ]
 

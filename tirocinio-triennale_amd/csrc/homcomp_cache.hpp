@@ -50,6 +50,9 @@ struct AttendArgs {
     float *partial;             // of more than one split: [tile][kColumns][split][head_dim]
     float *partial_sums;        // [tile][kColumns][split][2]: exponent the part is relative to, sum
     int32_t columns;            // columns that a tile can have
+    int32_t wide_tiles;         // tiles of many columns that a sequence's rows can take, 0: not that kernel
+    int32_t tiles_in_wide;      // of kColumns: 4, 8 or 16
+    uint32_t *left_over;        // [sequence, head, wide tile][split]: 1 where the columns are left to the other kernel
     const float *prior;
     float *weights;
     uint64_t weight_stride;

@@ -85,8 +85,8 @@ int rows_call(bool store, const homcomp_cache *cache, void *k, void *v, int type
 
 // Shapes of an attention call: column tiles, parts, scratch memory.
 struct AttendPlan {
-    int tiles, columns, splits, split_records;
-    size_t partial_bytes, sums_bytes, lse_bytes;
+    int tiles, columns, splits, split_records, wide_tiles, tiles_in_wide;
+    size_t partial_bytes, sums_bytes, lse_bytes, left_bytes;
 };
 
 int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, int64_t slots, AttendPlan *p)
@@ -106,10 +106,17 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
     if (records > (most + 31) / 32) records = (most + 31) / 32;
     if (records < 1) records = 1;
     const int64_t units = (int64_t)c->n_seqs * c->kv_heads * p->tiles;
+    // more columns than a tile: records are unpacked once for up to 4, 8 or 16 tiles (rows of 256 values leave no room for two tiles
+    // a wave); 32-bit results need more than float16 values
+    if (p->tiles > 1 && t->type != HOMCOMP_F32) {
+        p->tiles_in_wide = p->tiles <= 4 ? 4 : (p->tiles <= 8 || nb == 8 ? 8 : 16);
+        p->wide_tiles = (p->tiles + p->tiles_in_wide - 1) / p->tiles_in_wide;
+    }
+    const int64_t groups = p->wide_tiles ? (int64_t)c->n_seqs * c->kv_heads * p->wide_tiles : units;   // workgroups without parts
     // eight workgroups for every compute unit, so that sequences of different lengths even out, but eight records at least for
     // every wave (and two where there is little in all)
-    int64_t splits = units ? (8 * kComputeUnits + units - 1) / units : 1;
-    const int64_t least = units * records >= 64 * kComputeUnits ? 8 : 2;
+    int64_t splits = groups ? ((p->wide_tiles ? 2 : 8) * kComputeUnits + groups - 1) / groups : 1;
+    const int64_t least = groups * records >= 64 * kComputeUnits ? 8 : 2;
     const int64_t fine = (records + least * hc::kAttendWaves - 1) / (least * hc::kAttendWaves);
     if (splits > fine) splits = fine;
     int64_t each = (records + splits - 1) / splits;
@@ -123,6 +130,7 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
         p->partial_bytes = parts * (size_t)(32 * nb) * sizeof(float);
         p->sums_bytes = parts * 2 * sizeof(float);
     }
+    if (p->wide_tiles) p->left_bytes = (size_t)groups * (size_t)p->splits * sizeof(uint32_t);
     if (t->d_weights && !t->d_lse) p->lse_bytes = (t->n_rows * (size_t)t->q_heads * sizeof(float) + 15) / 16 * 16;
     return HOMCOMP_OK;
 }
@@ -155,7 +163,7 @@ size_t homcomp_cache_attend_scratch(const homcomp_cache *cache, const homcomp_at
     int64_t slots = 0;
     AttendPlan p;
     if (!attention || shape_of(cache, &nb, &slots) || plan_attention(cache, attention, nb, slots, &p)) return 0;
-    return p.partial_bytes + p.sums_bytes + p.lse_bytes;
+    return p.partial_bytes + p.sums_bytes + p.lse_bytes + p.left_bytes;
 }
 
 int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t, void *stream)
@@ -177,7 +185,7 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t,
         if (!t->d_q || !t->d_out || t->d_q == t->d_out) return HOMCOMP_ERR_INVALID_ARG;
         if (!aligned(t->d_q, bytes_of(t->type)) || !aligned(t->d_out, bytes_of(t->type))) return HOMCOMP_ERR_ALIGNMENT;
     }
-    const size_t need = p.partial_bytes + p.sums_bytes + p.lse_bytes;
+    const size_t need = p.partial_bytes + p.sums_bytes + p.lse_bytes + p.left_bytes;
     if (need && (!t->d_scratch || t->scratch_bytes < need)) return HOMCOMP_ERR_INVALID_ARG;
     a.q = t->d_q;
     a.out = t->d_out;
@@ -199,6 +207,9 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t,
     a.partial = (float *)t->d_scratch;
     a.partial_sums = (float *)((uint8_t *)t->d_scratch + p.partial_bytes);
     a.columns = p.columns;
+    a.wide_tiles = p.wide_tiles;
+    a.tiles_in_wide = p.tiles_in_wide;
+    if (p.wide_tiles) a.left_over = (uint32_t *)((uint8_t *)t->d_scratch + p.partial_bytes + p.sums_bytes + p.lse_bytes);
     a.prior = t->d_prior;
     a.weights = t->d_weights;
     a.weight_stride = t->weight_stride;

@@ -125,6 +125,28 @@ __device__ __forceinline__ uint8_t *record_of(const CacheArgs &c, const int32_t 
     const uint64_t record = (((uint64_t)page * (uint32_t)c.kv_heads + (uint32_t)h) << (c.page_shift - 5)) + (in_page >> 5);
     return c.pages + record * record_bytes(nb);
 }
+// Page numbers of 64 records ahead, one a lane: records first, first + step, .. below `end`.  A wave reads them from its lanes; a scalar
+// load for every record would have its latency in the way of every wait for LDS.
+struct PagesAhead {
+    uint32_t page;   // of record first + step * (64 q + lane)
+    int first, step, end;
+    __device__ __forceinline__ void refill(const CacheArgs &c, int s, int it, int lane)
+    {
+        const int own = it + step * lane;
+        page = own < end ? (uint32_t)c.table[(uint64_t)s * c.table_stride + ((uint32_t)(own * kRecordSlots) >> c.page_shift)] : 0xffffffffu;
+    }
+    // Record `it`, null where the table names no page or it is at or beyond the end.  Calls take first, first + step, .. in turn.
+    __device__ __forceinline__ const uint8_t *next(const CacheArgs &c, int s, int h, int it, int lane, int nb)
+    {
+        const int k = (it - first) / step & 63;
+        if (k == 0) refill(c, s, it, lane);
+        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)page, k);
+        if (p >= c.n_pages || it >= end) return nullptr;
+        const uint32_t in_page = ((uint32_t)it << 5) & ((1u << c.page_shift) - 1u);
+        const uint64_t record = (((uint64_t)p * (uint32_t)c.kv_heads + (uint32_t)h) << (c.page_shift - 5)) + (in_page >> 5);
+        return c.pages + record * record_bytes(nb);
+    }
+};
 // Rows of a sequence: its first one and how many, inside 0 .. n_rows.
 __device__ __forceinline__ void rows_of(const int32_t *starts, int s, int n_rows, int *first, int *count)
 {
@@ -318,10 +340,13 @@ constexpr int weight_parts() { return TY == kF32 ? 3 : 2; }
 template <int NB, int NQ>
 struct Queries {
     f16x8 q[NB][NQ];    // values 32 b + 8 g .. + 7 of the column's row, scaled; where codes stand sixteen times as high by 1/16 more
-    bf16x8 sums;        // g-th part (of three) of the sums over each block, times 2^-24
+    bf16x8 sums;        // g-th part (of three) of the sums over each block, times what the codes are
     float factor;       // what turns a score into the exponent of a power of two
     int see_from, see_to;   // slots see_from <= j < see_to are seen
 };
+
+template <int NB, int NQ>
+__device__ __forceinline__ bool sees(const Queries<NB, NQ> &q, int slot) { return slot >= q.see_from && slot < q.see_to; }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }
 
@@ -345,7 +370,9 @@ __device__ __forceinline__ void split_bf16(const float *x, bf16x8 *out)
 }
 
 // column: row * group + head of the group, at or beyond `columns` none (it sees no slot).
-template <int NB, int TY, bool FINE>
+// How codes enter the products of the scores: see code_pairs; kWhole: as the numbers c themselves.
+enum : int { kLow = 0, kFine = 1, kWhole = 2 };
+template <int NB, int TY, int FORM>
 __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int first, int count, int length, int column, int g,
                                              Queries<NB, query_parts<TY>()> &r)
 {
@@ -373,14 +400,14 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
         for (int i = 0; i < 8; ++i) total += x[b][i] * up;
         total += __shfl_xor(total, 16, 64);
         total += __shfl_xor(total, 32, 64);
-        sums[b] = total * 0x1p-24f;
+        sums[b] = FORM == kWhole ? total : total * 0x1p-24f;
         float rest[8];
         for (int i = 0; i < 8; ++i) rest[i] = x[b][i] * up;
         for (int p = 0; p < NQ; ++p) {
             for (int i = 0; i < 8; ++i) {
                 const _Float16 part = (_Float16)rest[i];
                 rest[i] -= (float)part;
-                r.q[b][p][i] = FINE || (i & 2) ? (_Float16)((float)part * 0.0625f) : part;
+                r.q[b][p][i] = FORM == kFine || (FORM == kLow && (i & 2)) ? (_Float16)((float)part * 0.0625f) : part;
             }
         }
     }
@@ -388,7 +415,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
     split_bf16<3>(sums, parts);
     const bf16x8 none = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
     r.sums = g == 0 ? parts[0] : (g == 1 ? parts[1] : (g == 2 ? parts[2] : none));
-    r.factor = ldexpf(a.scale * kLog2e, 10 + e);
+    r.factor = ldexpf(a.scale * kLog2e, (FORM == kWhole ? -14 : 10) + e);
     const int at = length - count + row;
     r.see_to = !there ? 0 : (a.causal ? (at + 1 < length ? at + 1 : length) : length);
     r.see_from = a.window > 0 && at + 1 - a.window > 0 ? at + 1 - a.window : 0;
@@ -489,17 +516,16 @@ __device__ __forceinline__ u32x4 code_pairs(uint32_t w)
 
 // x[T][r]: the score, short of `factor`, of slot 8 g + 4 T + r of the record for the lane's column.
 template <int NB, int NQ, bool FINE>
-__device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Queries<NB, NQ> &q, f32x4 (&x)[2])
+__device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Queries<NB, NQ> &q, const f32x4 &zero, f32x4 (&x)[2])
 {
     f32x4 part[2][NB];
     for (int T = 0; T < 2; ++T) {
         u32x4 lo = {0, 0, 0, 0};
         for (int i = 0; i < NB / 2; ++i) lo[i] = k.lows[T][i];
-        x[T] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), q.sums, f32x4{0, 0, 0, 0}, 0, 0, 0);
+        x[T] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), q.sums, zero, 0, 0, 0);
         for (int b = 0; b < NB; ++b) {
             const f16x8 c = __builtin_bit_cast(f16x8, code_pairs<FINE>(k.codes[T][b]));
-            part[T][b] = f32x4{0, 0, 0, 0};
-            for (int p = 0; p < NQ; ++p) part[T][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, q.q[b][p], part[T][b], 0, 0, 0);
+            for (int p = 0; p < NQ; ++p) part[T][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, q.q[b][p], p ? part[T][b] : zero, 0, 0, 0);
         }
     }
     for (int T = 0; T < 2; ++T)
@@ -508,10 +534,11 @@ __device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Querie
 }
 
 // Records that a tile's columns can see at all: [*from, *to).
+template <int COLUMNS = kColumns>
 __device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int length, int tile, int *from, int *to)
 {
-    const int first_row = tile * kColumns / a.group;
-    int last_row = (tile * kColumns + kColumns - 1) / a.group;
+    const int first_row = tile * COLUMNS / a.group;
+    int last_row = (tile * COLUMNS + COLUMNS - 1) / a.group;
     if (last_row >= count) last_row = count - 1;
     int end = length, begin = 0;
     if (a.causal && length - count + last_row + 1 < end) end = length - count + last_row + 1;
@@ -521,10 +548,11 @@ __device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int
     *to = begin < end ? (end + 31) >> 5 : begin >> 5;
 }
 // Slots that every one of a tile's columns sees: [*from, *to).
+template <int COLUMNS = kColumns>
 __device__ __forceinline__ void seen_by_all(const AttendArgs &a, int count, int length, int tile, int *from, int *to)
 {
-    const int first_row = tile * kColumns / a.group;
-    int last_row = (tile * kColumns + kColumns - 1) / a.group;
+    const int first_row = tile * COLUMNS / a.group;
+    int last_row = (tile * COLUMNS + COLUMNS - 1) / a.group;
     if (last_row >= count) last_row = count - 1;
     *to = a.causal && length - count + first_row + 1 < length ? length - count + first_row + 1 : length;
     *from = a.window > 0 && length - count + last_row + 1 - a.window > 0 ? length - count + last_row + 1 - a.window : 0;
@@ -557,30 +585,30 @@ struct Gathered {
 
 // One record.  A new reference exponent costs a multiplication of everything gathered, so it is taken only where a weight
 // would exceed 2^8 (32-bit sums have room for that); a lane looks at its own eight slots alone, and lanes exchange only then.
-template <int NB, int NQ, int NP, bool FINE, bool MASKED>
-__device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<NB, NQ> &q, int lane, int slot0, int length, Gathered<NB> &s)
+template <int NB, int NQ, int NP, bool FINE>
+__device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<NB, NQ> &q, int lane, int slot0, int length, bool masked, const f32x4 &zero, Gathered<NB> &s)
 {
     f32x4 x[2];
     KeyPart<NB> k;
     take_keys<NB>(at, lane, k);
-    record_scores<NB, NQ, FINE>(k, q, x);
+    record_scores<NB, NQ, FINE>(k, q, zero, x);
     ValuePart<NB> v;
     take_values<NB>(at, lane, v);
     // 2^64 goes in with the exponent, except for 32-bit results: next to 64 an exponent keeps 2^-19, too little for them
     constexpr float kUp = NP == 3 ? 0.0f : 64.0f;
-    float e[8];
-    bool seen[8];
+    float e[8], most = kNegInf;
     const float bias = kUp - s.top;      // (nothing seen yet: +infinity, which asks for a reference)
-    float most = kNegInf;
-    for (int i = 0; i < 8; ++i) {
-        seen[i] = !MASKED || (slot0 + i >= q.see_from && slot0 + i < q.see_to);
-        e[i] = seen[i] ? fmaf(x[i >> 2][i & 3], q.factor, bias) : kNegInf;
-        most = fmaxf(most, e[i]);
+    for (int i = 0; i < 8; ++i) e[i] = fmaf(x[i >> 2][i & 3], q.factor, bias);
+    if (masked) {
+        int from = slot0;
+        asm volatile("" : "+v"(from));   // (the comparisons stay under the branch)
+        for (int i = 0; i < 8; ++i) e[i] = sees(q, from + i) ? e[i] : kNegInf;
     }
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, e[i]);
     if (__builtin_amdgcn_ballot_w64(most > kUp + 8.0f) != 0) {
         most = kNegInf;
         for (int i = 0; i < 8; ++i)
-            if (seen[i]) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
+            if (!masked || sees(q, slot0 + i)) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
         const float now = fmaxf(s.top, most);
@@ -592,7 +620,7 @@ __device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<N
             for (int i = 0; i < NB / 2; ++i)
                 for (int n = 0; n < 4; ++n) s.o[i][n][r] *= shrink;
         }
-        for (int i = 0; i < 8; ++i) e[i] = seen[i] ? fmaf(x[i >> 2][i & 3], q.factor, kUp - now) : kNegInf;
+        for (int i = 0; i < 8; ++i) e[i] = !masked || sees(q, slot0 + i) ? fmaf(x[i >> 2][i & 3], q.factor, kUp - now) : kNegInf;
     }
     float p[8];
     for (int i = 0; i < 8; ++i) {
@@ -609,9 +637,11 @@ __device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<N
         for (int i = 0; i < 8; ++i) {
             const float step = (float)__builtin_bit_cast(f16x8, v.own_steps)[i];
             mid[i] = fmaf(step, (i & 1) ? 7.0f : 8.0f, (i & 1) ? __builtin_bit_cast(float, v.lows[i >> 1] & 0xffff0000u) : bf16_to_f32(v.lows[i >> 1]));
-            // a slot that only some columns see, or none: a NaN there reaches those that see it by p s_b
-            if (MASKED && (slot0 + i >= length || !(step == step))) mid[i] = 0.0f;
         }
+        // slots that only some columns see, or none: a NaN there reaches those that see it by p s_b
+        if (masked)
+            for (int i = 0; i < 8; ++i)
+                if (slot0 + i >= length || !(mid[i] == mid[i])) mid[i] = 0.0f;
         bf16x8 parts[NP];
         split_bf16<NP>(mid, parts);
         for (int n = 0; n < NP; ++n) middle[n] = __builtin_bit_cast(u32x4, parts[n]);
@@ -623,7 +653,12 @@ __device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<N
             s.low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, middle[n]), w[e2], s.low, 0, 0, 0);
     for (int b = 0; b < NB; ++b) {
         float ps[8];
-        for (int i = 0; i < 8; ++i) ps[i] = seen[i] ? fmaf((float)v.steps[b][i], p[i], 0.0f) : 0.0f;
+        for (int i = 0; i < 8; ++i) ps[i] = fmaf((float)v.steps[b][i], p[i], 0.0f);
+        if (masked) {
+            int from = slot0;
+            asm volatile("" : "+v"(from));
+            for (int i = 0; i < 8; ++i) ps[i] = sees(q, from + i) ? ps[i] : 0.0f;
+        }
         split_bf16<NP>(ps, w);
         const u32x4 codes = v.codes[b >> 1];
         constexpr bool kFineValues = NP == 3;
@@ -657,6 +692,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     const int tile = (int)(unit % (unsigned)a.tiles);
     const int h = (int)(unit / (unsigned)a.tiles % (unsigned)a.c.kv_heads);
     const int s = (int)(unit / (unsigned)a.tiles / (unsigned)a.c.kv_heads);
+    if (a.left_over && a.left_over[(unit / (unsigned)a.tiles * (unsigned)a.wide_tiles + (unsigned)(tile / a.tiles_in_wide)) * (unsigned)a.splits + (unsigned)split] == 0) return;
     int first, count;
     rows_of(a.starts, s, a.n_rows, &first, &count);
     const int length = sequence_length(a.c, s);
@@ -671,7 +707,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
 
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     Queries<NB, NQ> q;
-    load_queries<NB, TY, FINE>(a, h, first, count, length, tile * kColumns + n, g, q);
+    load_queries<NB, TY, FINE ? kFine : kLow>(a, h, first, count, length, tile * kColumns + n, g, q);
     Gathered<NB> acc;
     acc.low = f32x4{0, 0, 0, 0};
     for (int i = 0; i < NB / 2; ++i)
@@ -679,20 +715,21 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     acc.top = kNegInf;
     acc.total = 0.0f;
     uint8_t *stage = s_mem + wave * (int)record_bytes(NB);
+    f32x4 zero = {0, 0, 0, 0};
+    asm volatile("" : "+v"(zero));   // a register of zeros for the products to start from, instead of one cleared for each
     RawRecord<NB> raw;
     int it = from + wave;
-    const uint8_t *rec = it < to ? record_of(a.c, a.c.table, a.c.table_stride, s, h, it * kRecordSlots, NB) : nullptr;
+    PagesAhead pages = {0, it, kAttendWaves, to};
+    const uint8_t *rec = pages.next(a.c, s, h, it, lane, NB);
     if (rec) load_record<NB>(rec, lane, raw);
     while (it < to) {
         const int next = it + kAttendWaves;
-        const uint8_t *next_rec = next < to ? record_of(a.c, a.c.table, a.c.table_stride, s, h, next * kRecordSlots, NB) : nullptr;
+        const uint8_t *next_rec = pages.next(a.c, s, h, next, lane, NB);
         if (rec) lay_record<NB>(stage, lane, raw);
         if (next_rec) load_record<NB>(next_rec, lane, raw);
         if (rec) {
-            if (it * kRecordSlots >= all_from && (it + 1) * kRecordSlots <= all_to)
-                attend_record<NB, NQ, NP, FINE, false>(stage, q, lane, it * kRecordSlots + 8 * g, length, acc);
-            else
-                attend_record<NB, NQ, NP, FINE, true>(stage, q, lane, it * kRecordSlots + 8 * g, length, acc);
+            attend_record<NB, NQ, NP, FINE>(stage, q, lane, it * kRecordSlots + 8 * g, length,
+                                            it * kRecordSlots < all_from || (it + 1) * kRecordSlots > all_to, zero, acc);
         }
         it = next;
         rec = next_rec;
@@ -739,6 +776,329 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
         }
     } else {
         write_result<NB, TY>(a, h, first, tile * kColumns + column, part, all, sum, x);
+    }
+}
+
+// ---------------------------------------------------------------- attention of many rows
+//
+// With more columns than one tile the records are unpacked once for all of them.  A workgroup of W waves takes 16 CT W columns; all threads
+// together unpack records into LDS, ahead of the products, as float16 numbers: keys in two parts (22 bits: scores are exponents, and lse
+// is a 32-bit result), values in one.  That rounding, and the one of p to float16 (in two parts for float16
+// results), need numbers within float16's range.  A record with a NaN, or with blocks too large or too small for it, is not for this kernel:
+// the workgroup notes so, and k_cache_attend does its columns afterwards.
+//
+// Vector and matrix instructions about balance: for a record and 16 columns 8 multiply-adds, 8 exponentials (four times the cost
+// of others) and 25 more against 24 products of 16 cycles.  (With whole codes as keys, their scores scaled in 32 bits as above, it was 64 more
+// vector instructions for 8 products less, and 1410 us instead of what the table says for 2 x 2048 rows over 10007 slots.)
+template <int NB>
+struct WideRecord {
+    static constexpr uint32_t kRest = 2048u * NB, kValues = 4096u * NB, kBytes = 6144u * NB;   // keys from 0, their second parts
+    // steps and lowest numbers, as a record has them from kKeySteps on
+    static constexpr uint32_t kSides = 256u * NB, kVSteps = 64u * NB, kKLows = 128u * NB, kVLows = 192u * NB;
+    static constexpr int kPerStep = NB == 8 ? 1 : 2;   // records of a step: two steps fit into LDS
+};
+
+// A unit of unpacking work, a wave's: keys of blocks 2 half, 2 half + 1 of sixteen slots (unit = T * NB / 2 + half), or values 64 i + 32 half .. + 31
+// (unit = NB + 2 i + half).
+template <int NB>
+__device__ __forceinline__ u32x4 load_unit(const uint8_t *rec, int unit, int lane)
+{
+    const int m = lane & 15, g = lane >> 4;
+    u32x4 codes = {0, 0, 0, 0};
+    if (unit < NB) {
+        const int T = unit / (NB / 2), half = unit % (NB / 2), key = 8 * (m >> 2) + 4 * T + (m & 3);
+        const u32x2 w = *(const u32x2 *)(rec + key * 16 * NB + g * 4 * NB + half * 8);
+        codes[0] = w[0];
+        codes[1] = w[1];
+    } else {
+        codes = *(const u32x4 *)(rec + kValueCodes * NB + g * 128 * NB + (((unit - NB) >> 1) * 16 + m) * 16);
+    }
+    return codes;
+}
+// Two codes as float16 numbers: at bits 0 .. 3 under 1024, at bits 4 .. 7 under 64, both exact.
+__device__ __forceinline__ f16x2 codes_at_0(uint32_t w) { return __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u) - (_Float16)1024.0f; }
+__device__ __forceinline__ f16x2 codes_at_4(uint32_t w) { return __builtin_bit_cast(f16x2, (w & 0x00f000f0u) | 0x54005400u) - (_Float16)64.0f; }
+
+__device__ __forceinline__ f16x2 fma_pair(f16x2 a, f16x2 b, f16x2 c) { return __builtin_elementwise_fma(a, b, c); }
+
+// Halves of a word that belong to slots in front of `left`: slots 8 g + 2 n and 8 g + 2 n + 1.
+__device__ __forceinline__ uint32_t held_halves(int g, int n, int left)
+{
+    return (8 * g + 2 * n < left ? 0x0000ffffu : 0u) | (8 * g + 2 * n + 1 < left ? 0xffff0000u : 0u);
+}
+// Whether a block is for float16: s from 2^-13 to 2^11 and lo up to 2^15 in size; where s is 0, lo 0 or from 2^-13.
+__device__ __forceinline__ bool for_float16(uint32_t s, uint32_t lo)
+{
+    lo &= 0x7fffu;
+    return s <= 0x6800u && lo <= 0x4700u && (s >= 0x0800u || (s == 0 && (lo == 0 || lo >= 0x3900u)));
+}
+// Lays a unit into `at`; sides: the record's; left: slots of the record that the sequence holds (what lies behind counts for nothing).
+// False where a key's block is not for float16.
+template <int NB>
+__device__ __forceinline__ bool lay_unit(uint8_t *at, const uint8_t *sides, int unit, int lane, const u32x4 &codes, int left)
+{
+    const int m = lane & 15, g = lane >> 4;
+    if (unit < NB) {
+        const int T = unit / (NB / 2), half = unit % (NB / 2), key = 8 * (m >> 2) + 4 * T + (m & 3);
+        const uint32_t lows = *(const uint32_t *)(sides + WideRecord<NB>::kKLows + (key * NB + 2 * half) * 2);
+        bool fine = true;
+        for (int n = 0; n < 2; ++n) {
+            const uint32_t step = *(const uint16_t *)(sides + ((key >> 3) * NB + 2 * half + n) * 16 + (key & 7) * 2);
+            const uint32_t w = codes[n], high = w >> 8;
+            const float s = f16_to_f32(step), lo = n ? __builtin_bit_cast(float, lows & 0xffff0000u) : bf16_to_f32(lows & 0xffffu);
+            fine = fine && for_float16(step, (lows >> (16 * n)) & 0xffffu);
+            const f16x2 c[4] = {codes_at_0(w), codes_at_4(w), codes_at_0(high), codes_at_4(high)};
+            u32x4 first, rest;
+            for (int i = 0; i < 4; ++i) {
+                const float x = fmaf((float)c[i][0], s, lo), y = fmaf((float)c[i][1], s, lo);
+                const f16x2 k = {(_Float16)x, (_Float16)y};
+                const f16x2 r = {(_Float16)(x - (float)k[0]), (_Float16)(y - (float)k[1])};
+                first[i] = __builtin_bit_cast(uint32_t, k);
+                rest[i] = __builtin_bit_cast(uint32_t, r);
+            }
+            const int place = ((T * NB + 2 * half + n) * 64 + lane) * 16;
+            *(u32x4 *)(at + place) = first;
+            *(u32x4 *)(at + WideRecord<NB>::kRest + place) = rest;
+        }
+        return fine || key >= left;
+    }
+    const int i = (unit - NB) >> 1, half = (unit - NB) & 1;
+    u32x4 steps = *(const u32x4 *)(sides + WideRecord<NB>::kVSteps + (g * NB + unit - NB) * 16);
+    u32x4 lows = *(const u32x4 *)(sides + WideRecord<NB>::kVLows + (g * NB + unit - NB) * 16);
+    if (left < kRecordSlots) {
+        for (int n = 0; n < 4; ++n) {
+            steps[n] &= held_halves(g, n, left);
+            lows[n] &= held_halves(g, n, left);
+        }
+    }
+    u32x4 out[2];
+    for (int n = 0; n < 4; ++n) {
+        const uint32_t pair = steps[n];   // (a cast of the element in place takes the vector's first one)
+        const f16x2 s = __builtin_bit_cast(f16x2, pair);
+        const f16x2 lo = {(_Float16)bf16_to_f32(lows[n] & 0xffffu), (_Float16)__builtin_bit_cast(float, lows[n] & 0xffff0000u)};
+        const uint32_t w = half ? codes[n] >> 8 : codes[n];
+        out[0][n] = __builtin_bit_cast(uint32_t, fma_pair(codes_at_0(w), s, lo));
+        out[1][n] = __builtin_bit_cast(uint32_t, fma_pair(codes_at_4(w), s, lo));
+    }
+    for (int n = 0; n < 2; ++n) *(u32x4 *)(at + WideRecord<NB>::kValues + ((i * 4 + 2 * half + n) * 64 + lane) * 16) = out[n];
+    return true;
+}
+template <int NB>
+struct WideGathered {
+    f32x4 o[NB / 2][4];   // sum of value * p, values 64 i + 16 p + 4 g + r, times 2^7
+    float top, total;     // as in Gathered; total times 2^7
+};
+
+// The CT tiles of a wave together: what is read from LDS serves all of them.
+template <int NB, int CT, int NP>
+__device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB, 1> (&q)[CT], int lane, int slot0, bool masked, const f32x4 &zero, WideGathered<NB> (&s)[CT])
+{
+    f32x4 e[CT][2];   // exponents of slots slot0 + 4 T ..
+    for (int b = 0; b < NB; ++b) {
+        f16x8 k[2], rest[2];
+        for (int T = 0; T < 2; ++T) {
+            k[T] = *(const f16x8 *)(at + ((T * NB + b) * 64 + lane) * 16);
+            rest[T] = *(const f16x8 *)(at + WideRecord<NB>::kRest + ((T * NB + b) * 64 + lane) * 16);
+        }
+        for (int T = 0; T < 2; ++T)
+            for (int t = 0; t < CT; ++t) e[t][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest[T], q[t].q[b][0], b ? e[t][T] : zero, 0, 0, 0);
+        for (int T = 0; T < 2; ++T)
+            for (int t = 0; t < CT; ++t) e[t][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[T], q[t].q[b][0], e[t][T], 0, 0, 0);
+    }
+    bool higher = false;
+    for (int t = 0; t < CT; ++t) {
+        for (int i = 0; i < 8; ++i) e[t][i >> 2][i & 3] *= q[t].factor;
+        if (masked) {
+            int from = slot0;
+            asm volatile("" : "+v"(from));   // (the comparisons stay under the branch)
+            for (int i = 0; i < 8; ++i) e[t][i >> 2][i & 3] = sees(q[t], from + i) ? e[t][i >> 2][i & 3] : kNegInf;
+        }
+        float most = kNegInf;
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, e[t][i >> 2][i & 3]);
+        higher = higher || most > s[t].top + 8.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(higher) != 0) {
+        for (int t = 0; t < CT; ++t) {
+            float most = kNegInf;
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, e[t][i >> 2][i & 3]);
+            most = fmaxf(most, __shfl_xor(most, 16, 64));
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            const float now = fmaxf(s[t].top, most);
+            const float shrink = now == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(s[t].top - now);
+            s[t].top = now;
+            s[t].total *= shrink;
+            for (int i = 0; i < NB / 2; ++i)
+                for (int n = 0; n < 4; ++n)
+                    for (int r = 0; r < 4; ++r) s[t].o[i][n][r] *= shrink;
+        }
+    }
+    f16x8 w[CT][NP];
+    for (int t = 0; t < CT; ++t) {
+        const float bias = s[t].top == kNegInf ? 7.0f : 7.0f - s[t].top;
+        for (int i = 0; i < 8; ++i) {
+            const float p = __builtin_amdgcn_exp2f(e[t][i >> 2][i & 3] + bias);
+            s[t].total += p;
+            w[t][0][i] = (_Float16)p;
+            if (NP == 2) w[t][NP - 1][i] = (_Float16)(p - (float)w[t][0][i]);
+        }
+    }
+    for (int i = 0; i < NB / 2; ++i) {
+        for (int n = 0; n < 4; ++n) {
+            const f16x8 v = *(const f16x8 *)(at + WideRecord<NB>::kValues + ((i * 4 + n) * 64 + lane) * 16);
+            for (int t = 0; t < CT; ++t)
+                for (int k = 0; k < NP; ++k) s[t].o[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t][k], s[t].o[i][n], 0, 0, 0);
+        }
+    }
+}
+
+template <int NB, int TY, int W, int CT>
+__global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs a)
+{
+    constexpr int NP = TY == kF16 ? 2 : 1, D = 32 * NB, kWide = kColumns * CT * W;
+    constexpr int kPer = WideRecord<NB>::kPerStep, kUnits = (2 * kPer * NB + W - 1) / W;   // records of a step, units of a wave
+    __shared__ __align__(16) uint8_t s_mem[2][kPer][WideRecord<NB>::kBytes];
+    __shared__ __align__(16) uint8_t s_sides[2][kPer][WideRecord<NB>::kSides];
+    __shared__ uint32_t s_bad;
+    const uint32_t units = gridDim.x / (unsigned)a.splits;
+    const int split = (int)(blockIdx.x / units);
+    const uint32_t unit = blockIdx.x % units;    // (sequence, head, wide tile)
+    const int wide = (int)(unit % (unsigned)a.wide_tiles);
+    const int h = (int)(unit / (unsigned)a.wide_tiles % (unsigned)a.c.kv_heads);
+    const int s = (int)(unit / (unsigned)a.wide_tiles / (unsigned)a.c.kv_heads);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    if (threadIdx.x == 0) s_bad = 0;
+    int first, count;
+    rows_of(a.starts, s, a.n_rows, &first, &count);
+    const int length = sequence_length(a.c, s);
+    if (count > a.max_rows) count = a.max_rows;
+    if (wide * kWide >= count * a.group) return;
+    int from, to;
+    seen_records<kWide>(a, count, length, wide, &from, &to);
+    from += split * a.split_records;
+    if (to > from + a.split_records) to = from + a.split_records;
+
+    Queries<NB, 1> q[CT];
+    WideGathered<NB> acc[CT];
+    const int wave_tile = wide * W + wave;   // of 16 CT columns
+    int own_from, own_to, all_from, all_to;
+    seen_records<kColumns * CT>(a, count, length, wave_tile, &own_from, &own_to);
+    seen_by_all<kColumns * CT>(a, count, length, wave_tile, &all_from, &all_to);
+    if (wave_tile * kColumns * CT >= count * a.group) own_to = own_from;
+    for (int t = 0; t < CT; ++t) {
+        load_queries<NB, TY, kWhole>(a, h, first, count, length, (wave_tile * CT + t) * kColumns + n, g, q[t]);
+        acc[t].top = kNegInf;
+        acc[t].total = 0.0f;
+        for (int i = 0; i < NB / 2; ++i)
+            for (int p = 0; p < 4; ++p) acc[t].o[i][p] = f32x4{0, 0, 0, 0};
+    }
+
+    // Codes are unpacked a step ahead of the products, and loaded a step ahead of that, the sides another.  Of a step's two records, keys
+    // of the one and values of the other fall to the same wave.
+    const int steps = (to - from + kPer - 1) / kPer;
+    struct Pair {
+        const uint8_t *first, *second;
+        __device__ __forceinline__ const uint8_t *operator[](int r) const { return r ? second : first; }   // (an array would go to memory)
+    };
+    PagesAhead pages = {0, from, 1, to};
+    auto find = [&](int j) __attribute__((always_inline)) {   // (of j = 0, 1, .. in turn)
+        const int it = from + kPer * j;
+        const uint8_t *first = pages.next(a.c, s, h, it, lane, NB);
+        return Pair{first, kPer > 1 ? pages.next(a.c, s, h, it + 1, lane, NB) : nullptr};
+    };
+    u32x4 raw[kUnits], side = {0, 0, 0, 0};
+    const int side_rec = (int)threadIdx.x / (16 * NB), side_piece = (int)threadIdx.x % (16 * NB);
+    static_assert(64 * W >= 16 * kPer * NB, "a piece of the records' sides for every thread");
+    auto load_sides = [&](const Pair &p) __attribute__((always_inline)) {
+        const uint8_t *rec = p[side_rec];
+        if (side_rec < kPer && rec) side = *(const u32x4 *)(rec + kKeySteps * NB + side_piece * 16);
+    };
+    auto lay_sides = [&](int j) __attribute__((always_inline)) {
+        if (side_rec < kPer) *(u32x4 *)&s_sides[j & 1][side_rec][side_piece * 16] = side;
+    };
+    auto load_codes = [&](const Pair &p) __attribute__((always_inline)) {
+        for (int k = 0; k < kUnits; ++k) {
+            const int u = wave + k * W, r = u / (2 * NB);
+            const uint8_t *rec = p[r];
+            if (u < 2 * kPer * NB && rec) raw[k] = load_unit<NB>(rec, (u + r * NB) % (2 * NB), lane);
+        }
+    };
+    bool fine = true;
+    auto lay_codes = [&](int j, const Pair &p) __attribute__((always_inline)) {
+        for (int k = 0; k < kUnits; ++k) {
+            const int u = wave + k * W, r = u / (2 * NB);
+            if (u < 2 * kPer * NB && p[r])
+                fine = lay_unit<NB>(s_mem[j & 1][r], s_sides[j & 1][r], (u + r * NB) % (2 * NB), lane, raw[k], length - (from + kPer * j + r) * kRecordSlots) && fine;
+        }
+        // the values' blocks, one a thread
+        for (int k = 0; k < (32 * kPer * NB + 64 * W - 1) / (64 * W); ++k) {
+            const int n = (int)threadIdx.x + 64 * W * k, r = n / (32 * NB), block = n % (32 * NB), slot = block / (8 * NB) * 8 + block % 8;
+            if (r < kPer && p[r] && slot < length - (from + kPer * j + r) * kRecordSlots)
+                fine = fine && for_float16(*(const uint16_t *)&s_sides[j & 1][r][WideRecord<NB>::kVSteps + block * 2],
+                                           *(const uint16_t *)&s_sides[j & 1][r][WideRecord<NB>::kVLows + block * 2]);
+        }
+    };
+    f32x4 zero = {0, 0, 0, 0};
+    asm volatile("" : "+v"(zero));   // a register of zeros for the products to start from, instead of one cleared for each
+    Pair now = find(0), next = find(1), later = find(2);
+    load_sides(now);
+    load_codes(now);
+    lay_sides(0);
+    load_sides(next);
+    __syncthreads();
+    lay_codes(0, now);
+    lay_sides(1);
+    load_codes(next);
+    load_sides(later);
+    for (int j = 0; j < steps; ++j) {
+        __syncthreads();
+        lay_codes(j + 1, next);
+        lay_sides(j);   // (of step j + 2: those of step j are done with)
+        const Pair last = find(j + 3);
+        load_codes(later);
+        load_sides(last);
+#pragma unroll 1
+        for (int r = 0; r < kPer; ++r) {
+            const int at = from + kPer * j + r;
+            if (now[r] && at >= own_from && at < own_to)
+                attend_wide<NB, CT, NP>(s_mem[j & 1][r], q, lane, at * kRecordSlots + 8 * g, at * kRecordSlots < all_from || (at + 1) * kRecordSlots > all_to, zero, acc);
+        }
+        now = next;
+        next = later;
+        later = last;
+    }
+    if (!fine) s_bad = 1;
+    __syncthreads();
+    // (the kernel's first store: behind one, the table would no longer be read by scalar loads)
+    const bool left_over = s_bad != 0;
+    if (threadIdx.x == 0) a.left_over[unit * (unsigned)a.splits + (unsigned)split] = left_over ? 1 : 0;
+    if (left_over) return;
+    for (int t = 0; t < CT; ++t) {
+        const int tile = wave_tile * CT + t, column = tile * kColumns + n;
+        float total = acc[t].total;
+        total += __shfl_xor(total, 16, 64);
+        total += __shfl_xor(total, 32, 64);
+        total *= 0x1p-7f;
+        if (column >= count * a.group) continue;
+        const int row = column / a.group, head = column - row * a.group;
+        const uint64_t line = (uint64_t)(first + row) * a.out_row_stride + (uint64_t)(h * a.group + head) * a.out_head_stride;
+        const uint64_t place = (((uint64_t)(unit / (unsigned)a.wide_tiles) * (unsigned)a.tiles + (unsigned)tile) * kColumns + (unsigned)n) * (unsigned)a.splits + (unsigned)split;
+        const float scale = a.splits > 1 ? 0x1p-7f : (total == 0.0f ? 0.0f : 0x1p-7f / total);
+        for (int i = 0; i < NB / 2; ++i) {
+            for (int p = 0; p < 4; ++p) {
+                float v[4];
+                for (int r = 0; r < 4; ++r) v[r] = acc[t].o[i][p][r] * scale;
+                const uint64_t at = (uint64_t)(64 * i + 16 * p + 4 * g);
+                if (a.splits > 1) store_run<4, kF32>(a.partial, place * D + at, v);
+                else store_run<4, TY>(a.out, line + at, v);
+            }
+        }
+        if (g == 0 && a.splits > 1) {
+            a.partial_sums[2 * place] = acc[t].top;
+            a.partial_sums[2 * place + 1] = total;
+        } else if (g == 0 && a.lse) {
+            a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)] =
+                total == 0.0f ? kNegInf : (acc[t].top + __builtin_amdgcn_logf(total)) * kLn2;
+        }
     }
 }
 
@@ -874,7 +1234,7 @@ __global__ __launch_bounds__(256) void k_cache_weights(AttendArgs a, int records
         if (it0 + kHeldRecords <= from || it0 >= to) continue;
         const int column = tile * kColumns + n;
         Queries<NB, NQ> q;
-        load_queries<NB, TY, true>(a, h, first, count, length, column, g, q);
+        load_queries<NB, TY, kFine>(a, h, first, count, length, column, g, q);
         float lse = 0.0f;
         if (column < count * a.group) {
             const int row = column / a.group, head = column - row * a.group;
@@ -885,7 +1245,7 @@ __global__ __launch_bounds__(256) void k_cache_weights(AttendArgs a, int records
             KeyPart<NB> keys;
             take_keys<NB, 512, 576>(s_mem[wave][k], lane, keys);
             f32x4 x[2];
-            record_scores<NB, NQ, true>(keys, q, x);
+            record_scores<NB, NQ, true>(keys, q, f32x4{0, 0, 0, 0}, x);
             const int slot0 = (it0 + k) * kRecordSlots + 8 * g;
             for (int i = 0; i < 8; ++i)
                 if (slot0 + i >= q.see_from && slot0 + i < q.see_to)
@@ -1080,6 +1440,16 @@ static hipError_t attend_of(const AttendArgs &a, hipStream_t s)
     if (tiles) {
         // where weights are wanted the sums have to be those of the scores that they are taken from
         const dim3 grid(tiles * (uint32_t)a.splits);
+        if constexpr (TY != kF32) {
+            if (a.wide_tiles) {
+                const dim3 wide((uint32_t)a.c.n_seqs * (uint32_t)a.c.kv_heads * (uint32_t)a.wide_tiles * (uint32_t)a.splits);
+                if (a.tiles_in_wide == 4) hipLaunchKernelGGL((k_cache_attend_rows<NB, TY, 4, 1>), wide, dim3(256), 0, s, a);
+                else if (a.tiles_in_wide == 8) hipLaunchKernelGGL((k_cache_attend_rows<NB, TY, 8, 1>), wide, dim3(512), 0, s, a);
+                else if constexpr (NB < 8) hipLaunchKernelGGL((k_cache_attend_rows<NB, TY, 8, 2>), wide, dim3(512), 0, s, a);
+                e = hipGetLastError();
+                if (e != hipSuccess) return e;
+            }
+        }
         if (TY == kF32 || a.weights) hipLaunchKernelGGL((k_cache_attend<NB, TY, true>), grid, dim3(256), 0, s, a);
         else if constexpr (TY != kF32) hipLaunchKernelGGL((k_cache_attend<NB, TY, false>), grid, dim3(256), 0, s, a);
         e = hipGetLastError();
