@@ -12,6 +12,7 @@ refusal is a ValueError or a TypeError, and nothing has been enqueued then.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import _check, lib as _package_lib
 
@@ -21,24 +22,10 @@ EXPORTS = ("homcomp_cache_page_bytes", "homcomp_cache_store", "homcomp_cache_loa
 BF16, F16, F32 = 0, 1, 2
 
 
-class _CacheArgs(C.Structure):
-    _fields_ = [("d_pages", C.c_void_p), ("n_pages", C.c_size_t), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int),
-                ("n_seqs", C.c_int), ("d_table", C.c_void_p), ("table_stride", C.c_size_t), ("d_lengths", C.c_void_p)]
-
-
-class _AttentionArgs(C.Structure):
-    _fields_ = [("d_q", C.c_void_p), ("q_row_stride", C.c_size_t), ("q_head_stride", C.c_size_t),
-                ("d_out", C.c_void_p), ("out_row_stride", C.c_size_t), ("out_head_stride", C.c_size_t),
-                ("type", C.c_int), ("q_heads", C.c_int), ("d_starts", C.c_void_p), ("n_rows", C.c_size_t), ("max_rows", C.c_size_t),
-                ("max_length", C.c_size_t), ("scale", C.c_float), ("causal", C.c_int), ("window", C.c_size_t), ("d_lse", C.c_void_p),
-                ("d_prior", C.c_void_p), ("d_weights", C.c_void_p), ("weight_stride", C.c_size_t),
-                ("d_scratch", C.c_void_p), ("scratch_bytes", C.c_size_t)]
-
-
-class _EvictionArgs(C.Structure):
-    _fields_ = [("d_weights", C.c_void_p), ("weight_stride", C.c_size_t), ("max_length", C.c_size_t), ("keep", C.c_size_t),
-                ("first", C.c_size_t), ("recent", C.c_size_t), ("d_to_table", C.c_void_p), ("to_table_stride", C.c_size_t),
-                ("d_to_lengths", C.c_void_p), ("d_to_weights", C.c_void_p), ("d_kept", C.c_void_p)]
+# The argument structures of the header, packed by hand: a call's cost in Python is a good part of a small call's.
+_CACHE = struct.Struct("@P N iiii P N P")         # homcomp_cache
+_ATTENTION = struct.Struct("@P N N P N N ii P N N N f i N P P P N P N")   # homcomp_attention
+_EVICTION = struct.Struct("@P N N N N N P N P P P")                      # homcomp_eviction
 
 
 _lib = None
@@ -49,15 +36,15 @@ def lib() -> C.CDLL:
     global _lib
     if _lib is None:
         L = _package_lib()
-        vp, sz, cache = C.c_void_p, C.c_size_t, C.POINTER(_CacheArgs)
+        vp, sz = C.c_void_p, C.c_size_t   # (packed structures are bytes, which a void pointer takes)
         L.homcomp_cache_page_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
         L.homcomp_cache_page_bytes.restype = sz
         for name in ("homcomp_cache_store", "homcomp_cache_load"):
-            getattr(L, name).argtypes = [cache, vp, vp, C.c_int, sz, sz, vp, sz, vp]
-        L.homcomp_cache_attend_scratch.argtypes = [cache, C.POINTER(_AttentionArgs)]
+            getattr(L, name).argtypes = [vp, vp, vp, C.c_int, sz, sz, vp, sz, vp]
+        L.homcomp_cache_attend_scratch.argtypes = [vp, vp]
         L.homcomp_cache_attend_scratch.restype = sz
-        L.homcomp_cache_attend.argtypes = [cache, C.POINTER(_AttentionArgs), vp]
-        L.homcomp_cache_evict.argtypes = [cache, C.POINTER(_EvictionArgs), vp]
+        L.homcomp_cache_attend.argtypes = [vp, vp, vp]
+        L.homcomp_cache_evict.argtypes = [vp, vp, vp]
         _lib = L
     return _lib
 
@@ -79,16 +66,9 @@ def new_pages(n_pages: int, kv_heads: int, head_dim: int, page_tokens: int, devi
 
 def _stream_of(device, stream) -> int:
     import torch
-    return int((torch.cuda.current_stream(device) if stream is None else stream).cuda_stream)
-
-
-def _enqueue(device, call) -> int:
-    """Runs `call` with the tensors' device as the current one (the library launches there)."""
-    import torch
-    if device.type != "cuda" or device.index == torch.cuda.current_device():
-        return call()
-    with torch.cuda.device(device):
-        return call()
+    if stream is None:   # the handle alone, without the object around it: a tenth of the time
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return int(stream.cuda_stream)
 
 
 class Cache:
@@ -108,68 +88,82 @@ class Cache:
             raise ValueError(f"pages: contiguous uint8, a multiple of {self.page_bytes} bytes")
         self.pages, self.kv_heads, self.head_dim, self.page_tokens = pages, kv_heads, head_dim, page_tokens
         self.n_pages = pages.numel() // self.page_bytes
+        self._device = pages.device
         self._types = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
         self._int32, self._float32 = torch.int32, torch.float32
+        self._current_device = torch.cuda.current_device if pages.is_cuda else lambda: self._device.index
 
     # -- argument checks --------------------------------------------------------------------
+    def _call(self, name, function, *args):
+        """The call, with the pages' device as the current one (the library launches there)."""
+        if self._device.index == self._current_device():
+            status = function(*args)
+        else:
+            import torch
+            with torch.cuda.device(self._device):
+                status = function(*args)
+        if status:
+            _check(status, name)
+
     def _ints(self, name, t, dims):
-        if t.dtype is not self._int32 or t.dim() != dims or t.device != self.pages.device or (t.numel() and t.stride(-1) != 1):
-            raise ValueError(f"{name}: int32, {dims}-dimensional, adjacent numbers, on the pages' device")
-        return t
+        if t.dtype is not self._int32 or t.dim() != dims or t.device != self._device or not (t.is_contiguous() or not t.numel()):
+            raise ValueError(f"{name}: int32, {dims}-dimensional, contiguous, on the pages' device")
+        return t.data_ptr()
 
     def _args(self, table, lengths):
-        self._ints("table", table, 2)
-        self._ints("lengths", lengths, 1)
-        n = lengths.shape[0]
-        if table.shape[0] != n:
+        """The cache's structure for these sequences, how many they are and the pages that one can have."""
+        at, n_at = self._ints("table", table, 2), self._ints("lengths", lengths, 1)
+        n, width = table.shape
+        if lengths.shape[0] != n:
             raise ValueError("table: a row for every sequence")
-        if n > 1 and table.stride(0) != table.shape[1]:
-            raise ValueError("table: rows adjacent")
-        return _CacheArgs(self.pages.data_ptr(), self.n_pages, self.kv_heads, self.head_dim, self.page_tokens, n, table.data_ptr(),
-                          table.shape[1], lengths.data_ptr())
+        return _CACHE.pack(self.pages.data_ptr(), self.n_pages, self.kv_heads, self.head_dim, self.page_tokens, n, at, width, n_at), n, width
 
     def _starts(self, starts, n):
-        self._ints("starts", starts, 1)
+        at = self._ints("starts", starts, 1)
         if starts.shape[0] != n + 1:
             raise ValueError("starts: one number more than sequences")
-        return starts.data_ptr()
+        return at
 
     def _numbers(self, name, t, heads):
+        """Strides of rows and heads."""
         if t.dtype not in self._types:
             raise TypeError(f"{name}: bfloat16, float16 or float32")
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.device != self.pages.device:
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or t.device != self._device:
             raise ValueError(f"{name}: [rows, {heads}, {self.head_dim}] on the pages' device")
-        if t.numel() and (t.stride(2) != 1 or t.stride(0) < 0 or t.stride(1) < 0):
+        row, head, one = t.stride()
+        if one != 1 and t.numel():
             raise ValueError(f"{name}: the values of a row and head adjacent")
-        return t
+        return row, head
+
+    def _own_memory(self, name, t, row, head):
+        """Written tensors: no row or head of which shares another's memory."""
+        if t.numel() and (row == 0 and t.shape[0] > 1 or head == 0 and t.shape[1] > 1):
+            raise ValueError(f"{name}: rows and heads of its own memory")
 
     def _whole(self, name, t, shape, dtype):
-        if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != self.pages.device:
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.device != self._device:
             raise ValueError(f"{name}: contiguous {dtype} {list(shape)} on the pages' device")
         return t.data_ptr()
 
-    def _rows(self, name, what, k, v, table, lengths, starts, stream):
-        self._numbers("k", k, self.kv_heads)
-        self._numbers("v", v, self.kv_heads)
-        if k.dtype is not v.dtype or k.shape != v.shape or k.stride() != v.stride():
+    def _rows(self, name, what, written, k, v, table, lengths, starts, stream):
+        row, head = self._numbers("k", k, self.kv_heads)
+        if self._numbers("v", v, self.kv_heads) != (row, head) or k.dtype is not v.dtype or k.shape != v.shape:
             raise ValueError("k and v: of one type, shape and layout")
-        args = self._args(table, lengths)
-        first = self._starts(starts, args.n_seqs)
-        device = self.pages.device
-        _check(_enqueue(device, lambda: what(C.byref(args), k.data_ptr(), v.data_ptr(), self._types[k.dtype], k.stride(0), k.stride(1),
-                                             first, k.shape[0], _stream_of(device, stream))), name)
+        if written:
+            self._own_memory("k and v", k, row, head)
+        args, n, _ = self._args(table, lengths)
+        self._call(name, what, args, k.data_ptr(), v.data_ptr(), self._types[k.dtype], row, head, self._starts(starts, n), k.shape[0],
+                   _stream_of(self._device, stream))
 
     # -- the operators ----------------------------------------------------------------------
     def store(self, k, v, table, lengths, starts, stream=None) -> None:
         """Quantises the rows of k and v ([rows, kv_heads, head_dim]) into their slots."""
-        self._rows("cache_store", lib().homcomp_cache_store, k, v, table, lengths, starts, stream)
+        self._rows("cache_store", lib().homcomp_cache_store, False, k, v, table, lengths, starts, stream)
 
     def load(self, k, v, table, lengths, starts, stream=None) -> None:
         """Fills k and v with the rows that the slots stand for (of every sequence the last starts[s + 1] - starts[s] ones)."""
-        for name, t in (("k", k), ("v", v)):
-            if t.numel() and (t.shape[0] > 1 and t.stride(0) == 0 or t.shape[1] > 1 and t.stride(1) == 0):
-                raise ValueError(f"{name}: rows and heads of its own memory")
-        self._rows("cache_load", lib().homcomp_cache_load, k, v, table, lengths, starts, stream)
+        self._rows("cache_load", lib().homcomp_cache_load, True, k, v, table, lengths, starts, stream)
 
     def attend(self, q, out, table, lengths, starts, scale: float | None = None, causal: bool = True, window: int = 0,
                max_rows: int | None = None, max_length: int | None = None, lse=None, weights=None, prior=None, scratch=None,
@@ -183,69 +177,65 @@ class Cache:
         lse         float32 [rows, heads]: the log of the sum of the exponentials
         weights     float32 [sequences, kv_heads, at least max_length]: prior (same shape, may be weights, default 0) + the attention
                     that the slots received in this call
-        scratch     uint8, at least scratch_bytes(...) of them, not shared by calls that may overlap; by default memory of torch's
-                    allocator, taken for this call
+        scratch     at least scratch_bytes(...) bytes of contiguous memory, not shared by calls that may overlap; by default memory of
+                    torch's allocator, taken for this call
         """
-        if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+        rows, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+        if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"q: [rows, a multiple of {self.kv_heads}, {self.head_dim}]")
-        heads = q.shape[1]
-        self._numbers("q", q, heads)
-        self._numbers("out", out, heads)
+        q_row, q_head = self._numbers("q", q, heads)
+        out_row, out_head = self._numbers("out", out, heads)
         if out.dtype is not q.dtype or out.shape != q.shape:
             raise ValueError("out: of q's type and shape")
-        if out.numel() and (out.shape[0] > 1 and out.stride(0) == 0 or out.stride(1) == 0 and heads > 1):
-            raise ValueError("out: rows and heads of its own memory")
-        args = self._args(table, lengths)
-        t = self._attention(q, out, args, self._starts(starts, args.n_seqs), scale, causal, window, max_rows, max_length, lse, weights, prior)
+        self._own_memory("out", out, out_row, out_head)
+        args, n, width = self._args(table, lengths)
+        first = self._starts(starts, n)
+        most = width * self.page_tokens
+        max_length = most if max_length is None or max_length > most else max_length
+        max_rows = rows if max_rows is None or max_rows > rows else max_rows
+        if max_length < 0 or max_rows < 0 or window < 0:
+            raise ValueError("max_rows, max_length and window are not negative")
+        at_lse = self._whole("lse", lse, (rows, heads), self._float32) if lse is not None else None
+        at_weights = at_prior = None
+        stride = 0
+        if weights is not None:
+            stride = weights.shape[2] if weights.dim() == 3 else -1
+            if stride < max_length:
+                raise ValueError(f"weights: [sequences, kv_heads, at least max_length = {max_length}]")
+            at_weights = self._whole("weights", weights, (n, self.kv_heads, stride), self._float32)
+            if prior is not None:
+                at_prior = self._whole("prior", prior, (n, self.kv_heads, stride), self._float32)
+        elif prior is not None:
+            raise ValueError("prior goes with weights")
         L = lib()
-        need = L.homcomp_cache_attend_scratch(C.byref(args), C.byref(t))
+
+        def packed(memory, size):
+            return _ATTENTION.pack(q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head, self._types[q.dtype], heads, first, rows,
+                                   max_rows, max_length, self.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window,
+                                   at_lse or 0, at_prior or 0, at_weights or 0, stride, memory, size)
+
+        t = packed(0, 0)
+        need = L.homcomp_cache_attend_scratch(args, t)
         if need:
             if scratch is None:
                 scratch = q.new_empty((need + 3) // 4, dtype=self._float32)
                 if stream is not None:
                     scratch.record_stream(stream)
-            elif scratch.device != self.pages.device or not scratch.is_contiguous():
+            elif scratch.device != self._device or not scratch.is_contiguous():
                 raise ValueError("scratch: contiguous, on the pages' device")
-            t.d_scratch, t.scratch_bytes = scratch.data_ptr(), scratch.numel() * scratch.element_size()
-        device = self.pages.device
-        _check(_enqueue(device, lambda: L.homcomp_cache_attend(C.byref(args), C.byref(t), _stream_of(device, stream))), "cache_attend")
-
-    def _attention(self, q, out, args, first, scale, causal, window, max_rows, max_length, lse, weights, prior):
-        rows, heads = q.shape[0], q.shape[1]
-        most = args.table_stride * self.page_tokens
-        max_length = most if max_length is None else min(int(max_length), most)
-        max_rows = rows if max_rows is None else min(int(max_rows), rows)
-        if max_length < 0 or max_rows < 0 or window < 0:
-            raise ValueError("max_rows, max_length and window are not negative")
-        t = _AttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), self._types[q.dtype], heads,
-                           first, rows, max_rows, max_length, self.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window)
-        if lse is not None:
-            t.d_lse = self._whole("lse", lse, (rows, heads), self._float32)
-        if weights is None:
-            if prior is not None:
-                raise ValueError("prior goes with weights")
-            return t
-        for name, w in (("weights", weights), ("prior", prior)):
-            if w is not None and (w.dim() != 3 or w.shape[2] < max_length):
-                raise ValueError(f"{name}: [sequences, kv_heads, at least max_length = {max_length}]")
-        t.d_weights = self._whole("weights", weights, (args.n_seqs, self.kv_heads, weights.shape[2]), self._float32)
-        t.weight_stride = weights.shape[2]
-        if prior is not None:
-            t.d_prior = self._whole("prior", prior, weights.shape, self._float32)
-        return t
+            t = packed(scratch.data_ptr(), scratch.numel() * scratch.element_size())
+        self._call("cache_attend", L.homcomp_cache_attend, args, t, _stream_of(self._device, stream))
 
     def scratch_bytes(self, rows: int, heads: int, sequences: int, table_pages: int, dtype, window: int = 0, max_rows: int | None = None,
                       max_length: int | None = None, weights: bool = False, lse: bool = False) -> int:
         """Bytes of scratch memory that attend needs for these shapes."""
         most = table_pages * self.page_tokens
-        args = _CacheArgs(None, self.n_pages, self.kv_heads, self.head_dim, self.page_tokens, sequences, None, table_pages, None)
-        t = _AttentionArgs(type=self._types[dtype], q_heads=heads, n_rows=rows, max_rows=rows if max_rows is None else min(max_rows, rows),
-                           max_length=most if max_length is None else min(max_length, most), window=window)
-        if weights:
-            t.d_weights, t.weight_stride = 16, most   # (pointers are looked at for being there alone)
-        if lse:
-            t.d_lse = 16
-        return int(lib().homcomp_cache_attend_scratch(C.byref(args), C.byref(t)))
+        args = _CACHE.pack(0, self.n_pages, self.kv_heads, self.head_dim, self.page_tokens, sequences, 0, table_pages, 0)
+        # (pointers are looked at for being there alone)
+        t = _ATTENTION.pack(0, 0, 0, 0, 0, 0, self._types[dtype], heads, 0, rows, rows if max_rows is None else min(max_rows, rows),
+                            most if max_length is None else min(max_length, most), 1.0, 1, window, 16 if lse else 0, 0, 16 if weights else 0,
+                            most if weights else 0, 0, 0)
+        return int(lib().homcomp_cache_attend_scratch(args, t))
 
     def evict(self, weights, table, lengths, keep: int, to_table, to_lengths, first: int = 0, recent: int = 0,
               max_length: int | None = None, to_weights=None, kept=None, stream=None):
@@ -257,19 +247,18 @@ class Cache:
         to_table, to_lengths  where the rows go (the table is the caller's, its pages nobody's), and how many there are then
         to_weights, kept      [sequences, kv_heads, keep] float32 and int32: weights and old slots of the rows that stay
         """
-        args = self._args(table, lengths)
-        n = args.n_seqs
-        self._ints("to_table", to_table, 2)
-        if to_table.shape[0] != n or (n > 1 and to_table.stride(0) != to_table.shape[1]):
-            raise ValueError("to_table: a row for every sequence, rows adjacent")
-        most = table.shape[1] * self.page_tokens
-        max_length = most if max_length is None else min(int(max_length), most)
-        keep, first, recent = int(keep), int(first), int(recent)
+        args, n, width = self._args(table, lengths)
+        at_table = self._ints("to_table", to_table, 2)
+        if to_table.shape[0] != n:
+            raise ValueError("to_table: a row for every sequence")
+        most = width * self.page_tokens
+        max_length = most if max_length is None or max_length > most else max_length
         if keep < 1 or first < 0 or recent < 0 or first + recent > keep or max_length < 0:
             raise ValueError("keep is positive, first and recent are not negative and together at most keep")
         if keep > to_table.shape[1] * self.page_tokens:
             raise ValueError("to_table has no room for keep rows")
-        if weights.dim() != 3 or weights.shape[2] < max_length:
+        stride = weights.shape[2] if weights.dim() == 3 else -1
+        if stride < max_length:
             raise ValueError(f"weights: [sequences, kv_heads, at least max_length = {max_length}]")
         shape = (n, self.kv_heads, keep)
         to_weights = weights.new_empty(shape) if to_weights is None else to_weights
@@ -277,9 +266,8 @@ class Cache:
         if stream is not None:
             to_weights.record_stream(stream)
             kept.record_stream(stream)
-        t = _EvictionArgs(self._whole("weights", weights, (n, self.kv_heads, weights.shape[2]), self._float32), weights.shape[2], max_length,
-                          keep, first, recent, to_table.data_ptr(), to_table.shape[1], self._whole("to_lengths", to_lengths, (n,), self._int32),
-                          self._whole("to_weights", to_weights, shape, self._float32), self._whole("kept", kept, shape, self._int32))
-        device = self.pages.device
-        _check(_enqueue(device, lambda: lib().homcomp_cache_evict(C.byref(args), C.byref(t), _stream_of(device, stream))), "cache_evict")
+        t = _EVICTION.pack(self._whole("weights", weights, (n, self.kv_heads, stride), self._float32), stride, max_length, keep, first, recent, at_table,
+                           to_table.shape[1], self._whole("to_lengths", to_lengths, (n,), self._int32),
+                           self._whole("to_weights", to_weights, shape, self._float32), self._whole("kept", kept, shape, self._int32))
+        self._call("cache_evict", lib().homcomp_cache_evict, args, t, _stream_of(self._device, stream))
         return to_weights, kept

@@ -74,7 +74,7 @@ int rows_call(bool store, const homcomp_cache *cache, void *k, void *v, int type
     const int rc = cache_args(cache, SIZE_MAX, &c, &nb);
     if (rc) return rc;
     if (!type_ok(type)) return HOMCOMP_ERR_INVALID_ARG;
-    if (n_rows > (size_t)INT32_MAX || (int64_t)n_rows * cache->kv_heads * nb * 4 / 256 + 1 > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
+    if (n_rows > (size_t)INT32_MAX || ((int64_t)n_rows / 16 + 2 * (int64_t)cache->n_seqs) * cache->kv_heads > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
     if (c.n_seqs == 0 || n_rows == 0) return HOMCOMP_OK;
     if (!k || !v || !starts) return HOMCOMP_ERR_INVALID_ARG;
     if (!aligned(k, bytes_of(type)) || !aligned(v, bytes_of(type)) || !aligned(starts, 4)) return HOMCOMP_ERR_ALIGNMENT;

@@ -100,7 +100,7 @@ __device__ __forceinline__ void store_run(void *base, uint64_t at, const float *
     }
     for (int i = 0; i < N; ++i) store_number<TY>(base, at + (uint64_t)i, x[i]);
 }
-// N adjacent 32-bit numbers at a multiple of 16 bytes.
+// N adjacent 32-bit numbers, `at` of them on, at a multiple of 16 bytes.
 template <int N>
 __device__ __forceinline__ void load_run(const float *base, uint64_t at, float *x)
 {
@@ -148,27 +148,17 @@ struct PagesAhead {
     }
 };
 // Rows of a sequence: its first one and how many, inside 0 .. n_rows.
-__device__ __forceinline__ void rows_of(const int32_t *starts, int s, int n_rows, int *first, int *count)
+struct Rows {
+    int first, count;
+    int behind;    // rows from `first` to the sequence's last one, also those that are not there for us (n_rows, max_rows)
+};
+__device__ __forceinline__ Rows rows_of(const int32_t *starts, int s, int n_rows)
 {
     int a = starts[s], b = starts[s + 1];
     a = a < 0 ? 0 : (a > n_rows ? n_rows : a);
-    b = b < a ? a : (b > n_rows ? n_rows : b);
-    *first = a;
-    *count = b - a;
+    const int behind = b < a ? 0 : b - a;
+    return Rows{a, b > n_rows ? n_rows - a : behind, behind};
 }
-// The sequence that owns packed row `r`, -1 for padding: the last s with starts[s] <= r.
-__device__ __forceinline__ int sequence_of(const int32_t *starts, int n_seqs, int r)
-{
-    if (r < starts[0] || r >= starts[n_seqs]) return -1;
-    int lo = 0, hi = n_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid] <= r) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
 // ---------------------------------------------------------------- the codec
 struct Block8 {
     uint32_t code[8];   // of a lane's eight values
@@ -176,7 +166,8 @@ struct Block8 {
 };
 // Four adjacent lanes hold a block, eight values each.  All decisions are those of exact arithmetic: the borders lo + (j + 1/2) s
 // have at most 44 significant bits (s is at least a fifteenth of the range, lo at most 2^8 of its own last places), so 64-bit
-// floats hold them; a 32-bit estimate that is off by at most one is put right against them.
+// floats hold them.  In 32 bits (x - lo) / s + 1/2 is at most 15 1/2 and off by four roundings (the difference, the reciprocal, the product,
+// the sum): under 64 * 2^-24 = 2^-18.  Only where a value is within 2^-17 of a border, in about one wave of a hundred, are the borders looked at.
 __device__ __forceinline__ Block8 quantise(const float *x)
 {
     float mn = x[0], mx = x[0];
@@ -197,118 +188,221 @@ __device__ __forceinline__ Block8 quantise(const float *x)
     // toward minus infinity: cutting the low bits moves toward zero, a negative number that loses some goes one further
     const uint32_t bits = __builtin_bit_cast(uint32_t, mn);
     r.lo = (bits >> 16) + (((bits >> 31) != 0 && (bits & 0xffffu) != 0) ? 1u : 0u);
-    const double lo = (double)bf16_to_f32(r.lo), range = (double)mx - lo;
-    r.s = f32_to_f16((float)(range / 15.0));
+    const float lo = bf16_to_f32(r.lo);
+    const double range = (double)mx - (double)lo;
+    r.s = f32_to_f16((float)range * (1.0f / 15.0f));   // (within one place of the quotient: put right below, upward and down)
+    if ((r.s & 0x7fffu) < 0x7c00u && r.s > 0 && 15.0 * (double)f16_to_f32(r.s - 1) >= range) --r.s;
     if ((r.s & 0x7fffu) < 0x7c00u && 15.0 * (double)f16_to_f32(r.s) < range) ++r.s;
-    if (any || !(range <= 1.0e38) || (r.s & 0x7fffu) >= 0x7c00u) {
+    const bool none = any || !(range <= 1.0e38) || (r.s & 0x7fffu) >= 0x7c00u;
+    if (none) {
         r.s = 0x7e00u;
         r.lo = 0;
-        for (int i = 0; i < 8; ++i) r.code[i] = 0;
-        return r;
     }
-    const float sf = f16_to_f32(r.s), rs = sf > 0.0f ? 1.0f / sf : 0.0f, lof = (float)lo;
-    const double s = (double)sf;
+    const float s = f16_to_f32(r.s), rs = s > 0.0f ? 1.0f / s : 0.0f;
+    constexpr float near = 0x1p-17f;
+    float c[8];
+    bool close = false;
     for (int i = 0; i < 8; ++i) {
-        const float guess = fminf(fmaxf(floorf((x[i] - lof) * rs + 0.5f), 0.0f), 15.0f);
-        double c = (double)guess;
-        const double v = (double)x[i];
-        if (c < 15.0 && v >= fma(c + 0.5, s, lo)) c += 1.0;
-        else if (c > 0.0 && v < fma(c - 0.5, s, lo)) c -= 1.0;
-        r.code[i] = sf > 0.0f ? (uint32_t)(int)c : 0u;
+        const float t = (x[i] - lo) * rs + 0.5f, f = floorf(t);
+        c[i] = fminf(fmaxf(f, 0.0f), 15.0f);
+        close = close || !(t - f > near && t - f < 1.0f - near);
     }
+    if (close && s > 0.0f && !none) {
+        for (int i = 0; i < 8; ++i) {
+            const double v = (double)x[i], at = (double)c[i];
+            if (at < 15.0 && v >= fma(at + 0.5, (double)s, (double)lo)) c[i] += 1.0f;
+            else if (at > 0.0 && v < fma(at - 0.5, (double)s, (double)lo)) c[i] -= 1.0f;
+        }
+    }
+    for (int i = 0; i < 8; ++i) r.code[i] = s > 0.0f && !none ? (uint32_t)(int)c[i] : 0u;
     return r;
 }
 
-// Offsets of the parts of a record, in units of nb bytes.
+// Offsets of the parts of a record, in units of nb bytes (keys' codes at 0).
 constexpr uint32_t kValueCodes = 512, kKeySteps = 1024, kValueSteps = 1088, kKeyLows = 1152, kValueLows = 1216;
 
-// One row (32-bit numbers x[8] of a block in each four lanes): j is the lane's place in the block, t the slot in the record.
-__device__ __forceinline__ void write_key_block(uint8_t *rec, int nb, int t, int b, int j, const Block8 &q)
+// A wave takes 16 slots of one head that lie together in a record, as far as they belong to the batch's rows.  Work items: sequence s
+// begins at item starts[s] / 16 + 2 s, which leaves room for its rows however they lie to the sixteens.
+constexpr int kRowsOfWave = 16;
+
+struct RowsItem {
+    int s, h;           // sequence (-1: nothing to do) and head
+    int slot0;          // first slot, a multiple of 16
+    int begin, end;     // slots of it that are rows: slot0 + begin .. slot0 + end - 1
+    int row0;           // packed row of slot0 (may be in front of the first)
+};
+__device__ __forceinline__ RowsItem rows_item(const CacheArgs &c, const RowsArgs &a, uint32_t item)
 {
-    uint32_t w = 0;
-    for (int i = 0; i < 8; ++i) w |= q.code[i] << (4 * (i >> 1) + 16 * (i & 1));
-    *(uint32_t *)(rec + t * 16 * nb + j * 4 * nb + 4 * b) = w;
-    if (j == 0) {
-        *(uint16_t *)(rec + kKeySteps * nb + ((t >> 3) * nb + b) * 16 + (t & 7) * 2) = (uint16_t)q.s;
-        *(uint16_t *)(rec + kKeyLows * nb + (t * nb + b) * 2) = (uint16_t)q.lo;
+    RowsItem r = {-1, (int)(item % (uint32_t)c.kv_heads), 0, 0, 0, 0};
+    const int v = (int)(item / (uint32_t)c.kv_heads);
+    int lo = 0, hi = c.n_seqs;   // the last s with base(s) <= v
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        int at = a.starts[mid];
+        at = at < 0 ? 0 : (at > a.n_rows ? a.n_rows : at);
+        if ((at >> 4) + 2 * mid <= v) lo = mid;
+        else hi = mid;
     }
+    const Rows rows = rows_of(a.starts, lo, a.n_rows);
+    const int first = rows.first, count = rows.count, length = sequence_length(c, lo);
+    const int from = length - rows.behind;        // slot of the first row, in front of 0 where there are more rows than slots
+    const int begin = from > 0 ? from : 0;
+    const int last = from + count < length ? from + count : length;
+    const int group = (begin >> 4) + v - (first >> 4) - 2 * lo;
+    if (group < (begin >> 4) || group * kRowsOfWave >= last) return r;
+    r.s = lo;
+    r.slot0 = group * kRowsOfWave;
+    r.begin = begin > r.slot0 ? begin - r.slot0 : 0;
+    r.end = last - r.slot0 < kRowsOfWave ? last - r.slot0 : kRowsOfWave;
+    r.row0 = first + (r.slot0 - from);
+    return r;
 }
-// Values m and 16 + m of a block share a byte: lanes j and j ^ 2 exchange (all lanes of the wave take part), and lane j holds the bytes
-// m = 8 (j & 1) + 4 (j >> 1) + i afterwards.
-__device__ __forceinline__ void value_bytes(int j, const Block8 &q, uint32_t *bytes)
+__device__ __forceinline__ void wave_lds_order()
 {
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t give = j < 2 ? q.code[4 + i] : q.code[i];
-        const uint32_t got = (uint32_t)__shfl_xor((int)give, 2, 64);
-        bytes[i] = j < 2 ? q.code[i] | (got << 4) : got | (q.code[4 + i] << 4);
+    // a wave's LDS accesses take effect in order; this keeps the compiler from changing it
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Keys: four lanes to a slot, a lane's eight values of every block.  Values' codes of a slot lie two bytes at a time among those of seven others: the
+// wave gathers eight slots' words in LDS and writes them whole, except where not all eight are its own.
+template <int NB, int TY>
+__global__ __launch_bounds__(256) void k_cache_store(CacheArgs c, RowsArgs a, uint32_t items)
+{
+    __shared__ __align__(16) uint16_t s_words[4][2][8 * NB][8];   // [wave][octet][unit][slot]
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const uint32_t item = blockIdx.x * 4u + (uint32_t)wave;
+    if (item >= items) return;
+    const RowsItem r = rows_item(c, a, item);
+    if (r.s < 0) return;
+    uint8_t *rec = record_of(c, c.table, c.table_stride, r.s, r.h, r.slot0, NB);
+    if (!rec) return;
+    const int t = lane >> 2, j = lane & 3, slot = (r.slot0 & 31) + t;   // slot of the record
+    const bool own = t >= r.begin && t < r.end;
+    const uint64_t at = (uint64_t)(int64_t)(r.row0 + (own ? t : r.begin)) * a.row_stride + (uint64_t)r.h * a.head_stride + (uint64_t)(8 * j);
+    float x[NB][8];
+    for (int b = 0; b < NB; ++b) load8<TY>(a.k, at + (uint64_t)(32 * b), x[b]);
+#pragma unroll
+    for (int half = 0; half < (NB + 3) / 4; ++half) {
+        uint32_t w[4] = {0, 0, 0, 0}, step = 0, low = 0;
+        for (int n = 0; n < 4 && 4 * half + n < NB; ++n) {
+            const Block8 q = quantise(x[4 * half + n]);
+            for (int i = 0; i < 8; ++i) w[n] |= q.code[i] << (4 * (i >> 1) + 16 * (i & 1));
+            if (j == n) step = q.s, low = q.lo;
+        }
+        if (own) {
+            uint32_t *to = (uint32_t *)(rec + slot * 16 * NB + j * 4 * NB + 16 * half);
+            for (int n = 0; n < 4 && 4 * half + n < NB; ++n) to[n] = w[n];
+            const int b = 4 * half + j;   // a lane writes the scales of block j
+            if (b < NB) {
+                *(uint16_t *)(rec + kKeySteps * NB + ((slot >> 3) * NB + b) * 16 + (slot & 7) * 2) = (uint16_t)step;
+                *(uint16_t *)(rec + kKeyLows * NB + (slot * NB + b) * 2) = (uint16_t)low;
+            }
+        }
     }
-}
-__device__ __forceinline__ void write_value_block(uint8_t *rec, int nb, int t, int b, int j, const Block8 &q, const uint32_t *bytes)
-{
-    uint8_t *at = rec + kValueCodes * nb + (t >> 3) * 128 * nb + (t & 7) * 2 + (b & 1);
-    for (int i = 0; i < 4; ++i) at[((b >> 1) * 16 + 8 * (j & 1) + 4 * (j >> 1) + i) * 16] = (uint8_t)bytes[i];
-    if (j == 0) {
-        *(uint16_t *)(rec + kValueSteps * nb + ((t >> 3) * nb + b) * 16 + (t & 7) * 2) = (uint16_t)q.s;
-        *(uint16_t *)(rec + kValueLows * nb + ((t >> 3) * nb + b) * 16 + (t & 7) * 2) = (uint16_t)q.lo;
+    for (int b = 0; b < NB; ++b) load8<TY>(a.v, at + (uint64_t)(32 * b), x[b]);
+    uint32_t step[(NB + 3) / 4], low[(NB + 3) / 4];
+#pragma unroll
+    for (int i = 0; i < NB / 2; ++i) {
+        uint32_t word[4] = {0, 0, 0, 0};   // of units 16 i + 8 (j & 1) + 4 (j >> 1) + n
+        for (int e = 0; e < 2; ++e) {
+            const Block8 q = quantise(x[2 * i + e]);
+            // value m and value 16 + m of the block share a byte: lanes j and j ^ 2 exchange
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t give = j < 2 ? q.code[4 + n] : q.code[n];
+                const uint32_t got = (uint32_t)__shfl_xor((int)give, 2, 64);
+                word[n] |= (j < 2 ? q.code[n] | (got << 4) : got | (q.code[4 + n] << 4)) << (8 * e);
+            }
+            if (j == ((2 * i + e) & 3)) step[(2 * i + e) >> 2] = q.s, low[(2 * i + e) >> 2] = q.lo;
+        }
+        for (int n = 0; n < 4; ++n) s_words[wave][t >> 3][16 * i + 8 * (j & 1) + 4 * (j >> 1) + n][t & 7] = (uint16_t)word[n];
     }
-}
-__device__ __forceinline__ void read_key_block(const uint8_t *rec, int nb, int t, int b, int j, float *x)
-{
-    const uint32_t w = *(const uint32_t *)(rec + t * 16 * nb + j * 4 * nb + 4 * b);
-    const float s = f16_to_f32(*(const uint16_t *)(rec + kKeySteps * nb + ((t >> 3) * nb + b) * 16 + (t & 7) * 2));
-    const float lo = bf16_to_f32(*(const uint16_t *)(rec + kKeyLows * nb + (t * nb + b) * 2));
-    for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)((w >> (4 * (i >> 1) + 16 * (i & 1))) & 15u), lo);
-}
-__device__ __forceinline__ void read_value_block(const uint8_t *rec, int nb, int t, int b, int j, float *x)
-{
-    const uint8_t *at = rec + kValueCodes * nb + (t >> 3) * 128 * nb + (t & 7) * 2 + (b & 1);
-    const float s = f16_to_f32(*(const uint16_t *)(rec + kValueSteps * nb + ((t >> 3) * nb + b) * 16 + (t & 7) * 2));
-    const float lo = bf16_to_f32(*(const uint16_t *)(rec + kValueLows * nb + ((t >> 3) * nb + b) * 16 + (t & 7) * 2));
-    for (int i = 0; i < 8; ++i) {
-        const int m = 8 * (j & 1) + i;
-        x[i] = fmaf(s, (float)((at[((b >> 1) * 16 + m) * 16] >> (4 * (j >> 1))) & 15u), lo);
+    if (own) {
+        for (int half = 0; half < (NB + 3) / 4; ++half) {
+            const int b = 4 * half + j;
+            if (b < NB) {
+                *(uint16_t *)(rec + kValueSteps * NB + ((slot >> 3) * NB + b) * 16 + (slot & 7) * 2) = (uint16_t)step[half];
+                *(uint16_t *)(rec + kValueLows * NB + ((slot >> 3) * NB + b) * 16 + (slot & 7) * 2) = (uint16_t)low[half];
+            }
+        }
+    }
+    wave_lds_order();
+    for (int u = lane; u < 16 * NB; u += 64) {
+        const int o = u / (8 * NB), unit = u % (8 * NB);
+        const u32x4 words = *(const u32x4 *)s_words[wave][o][unit];
+        uint8_t *to = rec + kValueCodes * NB + (((r.slot0 & 31) >> 3) + o) * 128 * NB + unit * 16;
+        if (8 * o >= r.begin && 8 * o + 8 <= r.end) {
+            *(u32x4 *)to = words;
+        } else {
+            for (int n = 0; n < 8; ++n)
+                if (8 * o + n >= r.begin && 8 * o + n < r.end) ((uint16_t *)to)[n] = s_words[wave][o][unit][n];
+        }
     }
 }
 
-// Four lanes per block of 32 values of a row and head; every lane of a wave takes part in the exchanges, whether its row counts or not.
-template <int NB, int TY, bool STORE>
-__global__ __launch_bounds__(256) void k_cache_rows(CacheArgs c, RowsArgs a)
+// The mirror: keys straight to their rows, values through LDS, where rows come together.
+template <int NB, int TY>
+__global__ __launch_bounds__(256) void k_cache_load(CacheArgs c, RowsArgs a, uint32_t items)
 {
-    const uint64_t unit = ((uint64_t)blockIdx.x * 256 + threadIdx.x) >> 2;   // (row, head, block)
-    const int j = threadIdx.x & 3, b = (int)(unit % NB);
-    const uint64_t head_row = unit / NB;
-    const int h = (int)(head_row % (uint32_t)c.kv_heads);
-    const uint64_t row = head_row / (uint32_t)c.kv_heads;
-    int s = -1, slot = -1;
-    if (row < (uint64_t)a.n_rows) {
-        s = sequence_of(a.starts, c.n_seqs, (int)row);
-        if (s >= 0) {
-            const int n = sequence_length(c, s);
-            slot = n - (a.starts[s + 1] - (int)row);
-            if (slot < 0 || slot >= n) s = -1;
+    constexpr int D = 32 * NB, kSize = TY == kF32 ? 4 : 2;
+    __shared__ __align__(16) uint8_t s_rows[4][kRowsOfWave][D * kSize];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const uint32_t item = blockIdx.x * 4u + (uint32_t)wave;
+    if (item >= items) return;
+    const RowsItem r = rows_item(c, a, item);
+    if (r.s < 0) return;
+    const uint8_t *rec = record_of(c, c.table, c.table_stride, r.s, r.h, r.slot0, NB);
+    const int t = lane >> 2, j = lane & 3, slot = (r.slot0 & 31) + t;
+    const uint64_t head = (uint64_t)r.h * a.head_stride;
+    if (t >= r.begin && t < r.end) {
+        const uint64_t at = (uint64_t)(int64_t)(r.row0 + t) * a.row_stride + head + (uint64_t)(8 * j);
+        for (int b = 0; b < NB; ++b) {
+            float x[8];
+            for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+            if (rec) {
+                const uint32_t w = *(const uint32_t *)(rec + slot * 16 * NB + j * 4 * NB + 4 * b);
+                const float s = f16_to_f32(*(const uint16_t *)(rec + kKeySteps * NB + ((slot >> 3) * NB + b) * 16 + (slot & 7) * 2));
+                const float lo = bf16_to_f32(*(const uint16_t *)(rec + kKeyLows * NB + (slot * NB + b) * 2));
+                for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)((w >> (4 * (i >> 1) + 16 * (i & 1))) & 15u), lo);
+            }
+            store8<TY>(a.k, at + (uint64_t)(32 * b), x);
         }
     }
-    uint8_t *rec = s >= 0 ? record_of(c, c.table, c.table_stride, s, h, slot, NB) : nullptr;
-    const uint64_t at = row * a.row_stride + (uint64_t)h * a.head_stride + (uint64_t)(32 * b + 8 * j);
-    float x[8];
-    if (STORE) {
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-        if (rec) load8<TY>(a.k, at, x);
-        const Block8 key = quantise(x);
+    for (int u = lane; u < 16 * NB; u += 64) {
+        const int o = u / (8 * NB), unit = u % (8 * NB), i = unit >> 4, m = unit & 15, octet = ((r.slot0 & 31) >> 3) + o;
+        u32x4 words = {0, 0, 0, 0}, steps[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, lows[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         if (rec) {
-            write_key_block(rec, NB, slot & 31, b, j, key);
-            load8<TY>(a.v, at, x);
+            words = *(const u32x4 *)(rec + kValueCodes * NB + octet * 128 * NB + unit * 16);
+            for (int e = 0; e < 2; ++e) {
+                steps[e] = *(const u32x4 *)(rec + kValueSteps * NB + (octet * NB + 2 * i + e) * 16);
+                lows[e] = *(const u32x4 *)(rec + kValueLows * NB + (octet * NB + 2 * i + e) * 16);
+            }
         }
-        const Block8 value = quantise(x);
-        uint32_t bytes[4];
-        value_bytes(j, value, bytes);
-        if (rec) write_value_block(rec, NB, slot & 31, b, j, value, bytes);
-    } else if (s >= 0) {
-        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-        if (rec) read_key_block(rec, NB, slot & 31, b, j, x);
-        store8<TY>(a.k, at, x);
-        if (rec) read_value_block(rec, NB, slot & 31, b, j, x);
-        store8<TY>(a.v, at, x);
+        for (int n = 0; n < 8; ++n) {
+            const uint32_t word = words[n >> 1] >> (16 * (n & 1));
+            for (int p = 0; p < 4; ++p) {
+                const uint32_t step = steps[p >> 1][n >> 1], low = lows[p >> 1][n >> 1];
+                const float s = f16_to_f32((step >> (16 * (n & 1))) & 0xffffu);
+                const float lo = (n & 1) ? __builtin_bit_cast(float, low & 0xffff0000u) : bf16_to_f32(low & 0xffffu);
+                store_number<TY>(s_rows[wave][8 * o + n], (uint64_t)(64 * i + 16 * p + m), fmaf(s, (float)((word >> (4 * p)) & 15u), lo));
+            }
+        }
+    }
+    wave_lds_order();
+    constexpr int kPieces = D * kSize / 16;   // of a row
+    for (int u = lane; u < kRowsOfWave * kPieces; u += 64) {
+        const int row = u / kPieces, piece = u % kPieces;
+        if (row < r.begin || row >= r.end) continue;
+        const u32x4 v = *(const u32x4 *)(s_rows[wave][row] + piece * 16);
+        uint8_t *to = (uint8_t *)a.v + ((uint64_t)(int64_t)(r.row0 + row) * a.row_stride + head) * kSize + (uint64_t)(piece * 16);
+        if (((uintptr_t)to & 15u) == 0) {
+            *(u32x4 *)to = v;
+        } else if (TY == kF32) {
+            for (int n = 0; n < 4; ++n) ((uint32_t *)to)[n] = v[n];
+        } else {
+            for (int n = 0; n < 8; ++n) ((uint16_t *)to)[n] = (uint16_t)(v[n >> 1] >> (16 * (n & 1)));
+        }
     }
 }
 
@@ -373,7 +467,7 @@ __device__ __forceinline__ void split_bf16(const float *x, bf16x8 *out)
 // How codes enter the products of the scores: see code_pairs; kWhole: as the numbers c themselves.
 enum : int { kLow = 0, kFine = 1, kWhole = 2 };
 template <int NB, int TY, int FORM>
-__device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int first, int count, int length, int column, int g,
+__device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int first, int count, int slot0, int length, int column, int g,
                                              Queries<NB, query_parts<TY>()> &r)
 {
     constexpr int NQ = query_parts<TY>();
@@ -416,7 +510,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
     const bf16x8 none = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
     r.sums = g == 0 ? parts[0] : (g == 1 ? parts[1] : (g == 2 ? parts[2] : none));
     r.factor = ldexpf(a.scale * kLog2e, (FORM == kWhole ? -14 : 10) + e);
-    const int at = length - count + row;
+    const int at = slot0 + row;
     r.see_to = !there ? 0 : (a.causal ? (at + 1 < length ? at + 1 : length) : length);
     r.see_from = a.window > 0 && at + 1 - a.window > 0 ? at + 1 - a.window : 0;
 }
@@ -535,27 +629,27 @@ __device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Querie
 
 // Records that a tile's columns can see at all: [*from, *to).
 template <int COLUMNS = kColumns>
-__device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int length, int tile, int *from, int *to)
+__device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int slot0, int length, int tile, int *from, int *to)
 {
     const int first_row = tile * COLUMNS / a.group;
     int last_row = (tile * COLUMNS + COLUMNS - 1) / a.group;
     if (last_row >= count) last_row = count - 1;
     int end = length, begin = 0;
-    if (a.causal && length - count + last_row + 1 < end) end = length - count + last_row + 1;
-    if (a.window > 0 && length - count + first_row + 1 - a.window > 0) begin = length - count + first_row + 1 - a.window;
+    if (a.causal && slot0 + last_row + 1 < end) end = slot0 + last_row + 1;
+    if (a.window > 0 && slot0 + first_row + 1 - a.window > 0) begin = slot0 + first_row + 1 - a.window;
     if (end < 0) end = 0;
     *from = begin >> 5;
     *to = begin < end ? (end + 31) >> 5 : begin >> 5;
 }
 // Slots that every one of a tile's columns sees: [*from, *to).
 template <int COLUMNS = kColumns>
-__device__ __forceinline__ void seen_by_all(const AttendArgs &a, int count, int length, int tile, int *from, int *to)
+__device__ __forceinline__ void seen_by_all(const AttendArgs &a, int count, int slot0, int length, int tile, int *from, int *to)
 {
     const int first_row = tile * COLUMNS / a.group;
     int last_row = (tile * COLUMNS + COLUMNS - 1) / a.group;
     if (last_row >= count) last_row = count - 1;
-    *to = a.causal && length - count + first_row + 1 < length ? length - count + first_row + 1 : length;
-    *from = a.window > 0 && length - count + last_row + 1 - a.window > 0 ? length - count + last_row + 1 - a.window : 0;
+    *to = a.causal && slot0 + first_row + 1 < length ? slot0 + first_row + 1 : length;
+    *from = a.window > 0 && slot0 + last_row + 1 - a.window > 0 ? slot0 + last_row + 1 - a.window : 0;
 }
 
 // One column's share of a workgroup's result: out rows of 16 columns, 16 threads each.
@@ -693,21 +787,20 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     const int h = (int)(unit / (unsigned)a.tiles % (unsigned)a.c.kv_heads);
     const int s = (int)(unit / (unsigned)a.tiles / (unsigned)a.c.kv_heads);
     if (a.left_over && a.left_over[(unit / (unsigned)a.tiles * (unsigned)a.wide_tiles + (unsigned)(tile / a.tiles_in_wide)) * (unsigned)a.splits + (unsigned)split] == 0) return;
-    int first, count;
-    rows_of(a.starts, s, a.n_rows, &first, &count);
-    const int length = sequence_length(a.c, s);
-    if (count > a.max_rows) count = a.max_rows;
+    const Rows rows = rows_of(a.starts, s, a.n_rows);
+    const int first = rows.first, count = rows.count < a.max_rows ? rows.count : a.max_rows;
+    const int length = sequence_length(a.c, s), slot0 = length - rows.behind;   // slot of the first row (in front of 0: more rows than slots)
     if (tile * kColumns >= count * a.group) return;
     int from, to, all_from, all_to;
-    seen_records(a, count, length, tile, &from, &to);
-    seen_by_all(a, count, length, tile, &all_from, &all_to);
+    seen_records(a, count, slot0, length, tile, &from, &to);
+    seen_by_all(a, count, slot0, length, tile, &all_from, &all_to);
     from += split * a.split_records;
     if (split > 0 && from >= to) return;
     if (to > from + a.split_records) to = from + a.split_records;
 
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     Queries<NB, NQ> q;
-    load_queries<NB, TY, FINE ? kFine : kLow>(a, h, first, count, length, tile * kColumns + n, g, q);
+    load_queries<NB, TY, FINE ? kFine : kLow>(a, h, first, count, slot0, length, tile * kColumns + n, g, q);
     Gathered<NB> acc;
     acc.low = f32x4{0, 0, 0, 0};
     for (int i = 0; i < NB / 2; ++i)
@@ -967,13 +1060,12 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
     const int s = (int)(unit / (unsigned)a.wide_tiles / (unsigned)a.c.kv_heads);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     if (threadIdx.x == 0) s_bad = 0;
-    int first, count;
-    rows_of(a.starts, s, a.n_rows, &first, &count);
-    const int length = sequence_length(a.c, s);
-    if (count > a.max_rows) count = a.max_rows;
+    const Rows rows = rows_of(a.starts, s, a.n_rows);
+    const int first = rows.first, count = rows.count < a.max_rows ? rows.count : a.max_rows;
+    const int length = sequence_length(a.c, s), slot0 = length - rows.behind;   // slot of the first row (in front of 0: more rows than slots)
     if (wide * kWide >= count * a.group) return;
     int from, to;
-    seen_records<kWide>(a, count, length, wide, &from, &to);
+    seen_records<kWide>(a, count, slot0, length, wide, &from, &to);
     from += split * a.split_records;
     if (to > from + a.split_records) to = from + a.split_records;
 
@@ -981,11 +1073,11 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
     WideGathered<NB> acc[CT];
     const int wave_tile = wide * W + wave;   // of 16 CT columns
     int own_from, own_to, all_from, all_to;
-    seen_records<kColumns * CT>(a, count, length, wave_tile, &own_from, &own_to);
-    seen_by_all<kColumns * CT>(a, count, length, wave_tile, &all_from, &all_to);
+    seen_records<kColumns * CT>(a, count, slot0, length, wave_tile, &own_from, &own_to);
+    seen_by_all<kColumns * CT>(a, count, slot0, length, wave_tile, &all_from, &all_to);
     if (wave_tile * kColumns * CT >= count * a.group) own_to = own_from;
     for (int t = 0; t < CT; ++t) {
-        load_queries<NB, TY, kWhole>(a, h, first, count, length, (wave_tile * CT + t) * kColumns + n, g, q[t]);
+        load_queries<NB, TY, kWhole>(a, h, first, count, slot0, length, (wave_tile * CT + t) * kColumns + n, g, q[t]);
         acc[t].top = kNegInf;
         acc[t].total = 0.0f;
         for (int i = 0; i < NB / 2; ++i)
@@ -1115,13 +1207,12 @@ __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
     const int tile = (int)(unit % (unsigned)a.tiles);
     const int h = (int)(unit / (unsigned)a.tiles % (unsigned)a.c.kv_heads);
     const int s = (int)(unit / (unsigned)a.tiles / (unsigned)a.c.kv_heads);
-    int first, count;
-    rows_of(a.starts, s, a.n_rows, &first, &count);
-    const int length = sequence_length(a.c, s);
-    if (count > a.max_rows) count = a.max_rows;
+    const Rows rows = rows_of(a.starts, s, a.n_rows);
+    const int first = rows.first, count = rows.count < a.max_rows ? rows.count : a.max_rows;
+    const int length = sequence_length(a.c, s), slot0 = length - rows.behind;   // slot of the first row (in front of 0: more rows than slots)
     if (tile * kColumns + column >= count * a.group) return;
     int from, to;
-    seen_records(a, count, length, tile, &from, &to);
+    seen_records(a, count, slot0, length, tile, &from, &to);
     int parts = (to - from + a.split_records - 1) / a.split_records;
     if (parts < 1) parts = 1;
     if (parts > a.splits) parts = a.splits;
@@ -1208,10 +1299,9 @@ __global__ __launch_bounds__(256) void k_cache_weights(AttendArgs a, int records
     const int it0 = (int)(blockIdx.x % groups) * (kAttendWaves * kHeldRecords) + wave * kHeldRecords;
     const int h = (int)(blockIdx.x / groups % (unsigned)a.c.kv_heads);
     const int s = (int)(blockIdx.x / groups / (unsigned)a.c.kv_heads);
-    int first, count;
-    rows_of(a.starts, s, a.n_rows, &first, &count);
-    const int length = sequence_length(a.c, s);
-    if (count > a.max_rows) count = a.max_rows;
+    const Rows rows = rows_of(a.starts, s, a.n_rows);
+    const int first = rows.first, count = rows.count < a.max_rows ? rows.count : a.max_rows;
+    const int length = sequence_length(a.c, s), slot0 = length - rows.behind;   // slot of the first row (in front of 0: more rows than slots)
     if (it0 * kRecordSlots >= length) return;
     bool there[kHeldRecords];
     RawKeys<NB> raw[kHeldRecords];
@@ -1222,19 +1312,17 @@ __global__ __launch_bounds__(256) void k_cache_weights(AttendArgs a, int records
     }
     for (int k = 0; k < kHeldRecords; ++k)
         if (there[k]) lay_keys<NB>(s_mem[wave][k], lane, raw[k]);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_lds_order();
     float sum[kHeldRecords][8];
     for (int k = 0; k < kHeldRecords; ++k)
         for (int i = 0; i < 8; ++i) sum[k][i] = 0.0f;
     for (int tile = 0; tile * kColumns < count * a.group; ++tile) {
         int from, to;
-        seen_records(a, count, length, tile, &from, &to);
+        seen_records(a, count, slot0, length, tile, &from, &to);
         if (it0 + kHeldRecords <= from || it0 >= to) continue;
         const int column = tile * kColumns + n;
         Queries<NB, NQ> q;
-        load_queries<NB, TY, kFine>(a, h, first, count, length, column, g, q);
+        load_queries<NB, TY, kFine>(a, h, first, count, slot0, length, column, g, q);
         float lse = 0.0f;
         if (column < count * a.group) {
             const int row = column / a.group, head = column - row * a.group;
@@ -1246,9 +1334,9 @@ __global__ __launch_bounds__(256) void k_cache_weights(AttendArgs a, int records
             take_keys<NB, 512, 576>(s_mem[wave][k], lane, keys);
             f32x4 x[2];
             record_scores<NB, NQ, true>(keys, q, f32x4{0, 0, 0, 0}, x);
-            const int slot0 = (it0 + k) * kRecordSlots + 8 * g;
+            const int from_slot = (it0 + k) * kRecordSlots + 8 * g;
             for (int i = 0; i < 8; ++i)
-                if (slot0 + i >= q.see_from && slot0 + i < q.see_to)
+                if (sees(q, from_slot + i))
                     sum[k][i] += __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, lse * -kLog2e));
         }
     }
@@ -1273,8 +1361,8 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024;
-// Exclusive prefix of two counts per thread over the workgroup (a: low half, b: high half of one number, at most 1024 each).
+constexpr int kSelectThreads = 1024, kSelectEach = 16, kSelectTile = kSelectThreads * kSelectEach, kSelectBins = 2048;
+// Exclusive prefix of a count per thread over the workgroup.
 __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t *sums, uint32_t *all)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1296,10 +1384,12 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t *sums, 
     return before + x - mine;
 }
 
-// A workgroup per sequence and head finds the key of the last weight to stay, byte by byte from the top, then lists what stays in order.
+// A workgroup per sequence and head.  A thread holds sixteen neighbouring weights, so that ranks need one prefix sum over the threads; sequences
+// of up to 16384 slots are read once, longer ones once for each of the passes.  The key of the last weight to stay is found 11,
+// 11 and 10 bits at a time from the top: counts in LDS, then a prefix sum from the largest bin down.
 __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
 {
-    __shared__ uint32_t s_count[256];
+    __shared__ uint32_t s_bins[kSelectBins];
     __shared__ uint32_t s_sums[kSelectThreads / 64];
     __shared__ uint32_t s_found[2];
     const int h = (int)(blockIdx.x % (unsigned)a.c.kv_heads), s = (int)(blockIdx.x / (unsigned)a.c.kv_heads);
@@ -1307,103 +1397,141 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
     const uint64_t unit = (uint64_t)s * a.c.kv_heads + h;
     const float *w = a.weights + unit * a.weight_stride;
     const int count = length < a.keep ? length : a.keep;
-    if (h == 0 && tid == 0) a.to_lengths[s] = count;
     const bool all = length <= a.keep;
     const int low = a.first, high = length - a.recent;           // candidates: low <= slot < high
     uint32_t need = (uint32_t)(a.keep - a.first - a.recent);     // of them to stay
-    uint32_t key = 0xffffffffu;
-    if (!all && need > 0) {
-        uint32_t prefix = 0, mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s_count[tid] = 0;
+    const bool some = !all && need > 0, once = length <= kSelectTile;
+    float own[kSelectEach];
+    auto load = [&](int base) __attribute__((always_inline)) {
+        const int j = base + tid * kSelectEach;
+        if (j + kSelectEach <= length && ((uintptr_t)(w + j) & 15u) == 0) {
+            load_run<kSelectEach>(w, (uint64_t)j, own);
+        } else {
+            for (int i = 0; i < kSelectEach; ++i) own[i] = j + i < length ? w[j + i] : 0.0f;
+        }
+    };
+    load(0);
+    uint32_t prefix = 0, mask = 0;
+    if (some) {
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+            const uint32_t digits = pass == 2 ? 1023u : 2047u;
+            s_bins[tid] = 0;
+            s_bins[tid + kSelectThreads] = 0;
             __syncthreads();
-            for (int j = low + tid; j < high; j += kSelectThreads) {
-                const uint32_t k = weight_key(w[j]);
-                if ((k & mask) == prefix) atomicAdd(&s_count[(k >> shift) & 255u], 1u);
+            for (int base = 0; base < length; base += kSelectTile) {
+                if (!once) load(base);
+                for (int i = 0; i < kSelectEach; ++i) {
+                    const int j = base + tid * kSelectEach + i;
+                    const uint32_t k = weight_key(own[i]);
+                    if (j >= low && j < high && (k & mask) == prefix) atomicAdd(&s_bins[(k >> shift) & digits], 1u);
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                uint32_t left = need;
-                int digit = 255;
-                while (digit > 0 && s_count[digit] < left) left -= s_count[digit--];
-                s_found[0] = (uint32_t)digit;
-                s_found[1] = left;
+            const uint32_t bin = (uint32_t)(kSelectBins - 1 - 2 * tid), c0 = s_bins[bin], c1 = s_bins[bin - 1];
+            uint32_t total;
+            const uint32_t before = block_prefix(c0 + c1, s_sums, &total);
+            if (before < need && need <= before + c0 + c1) {
+                const bool second = need > before + c0;
+                s_found[0] = second ? bin - 1 : bin;
+                s_found[1] = need - before - (second ? c0 : 0u);
             }
             __syncthreads();
             prefix |= s_found[0] << shift;
-            mask |= 255u << shift;
+            mask |= digits << shift;
             need = s_found[1];
             __syncthreads();
         }
-        key = prefix;   // `need` of the weights with this key stay, those in front
     }
+    // all with a larger key than `prefix` stay, and `need` of those with that key, the ones in front
     uint32_t kept = 0, equal = 0;
-    for (int base = 0; base < length; base += kSelectThreads) {
-        const int j = base + tid;
-        const bool there = j < length, fixed = there && (all || j < low || j >= high);
-        const float weight = there ? w[j] : 0.0f;
-        const uint32_t k = weight_key(weight);
-        const bool same = there && !fixed && key != 0xffffffffu && k == key;
-        uint32_t total;
-        const uint32_t before = block_prefix(same ? 1u : 0u, s_sums, &total);
-        const bool stays = fixed || (there && !fixed && key != 0xffffffffu && (k > key || (same && equal + before < need)));
+    for (int base = 0; base < length; base += kSelectTile) {
+        if (!once) load(base);
+        const int j0 = base + tid * kSelectEach;
+        uint32_t same = 0, total;
+        for (int i = 0; i < kSelectEach; ++i)
+            if (some && j0 + i >= low && j0 + i < high && weight_key(own[i]) == prefix) same |= 1u << i;
+        uint32_t rank = equal + block_prefix((uint32_t)__builtin_popcount(same), s_sums, &total), stays = 0;
         equal += total;
-        const uint32_t at = block_prefix(stays ? 1u : 0u, s_sums, &total);
-        if (stays && kept + at < (uint32_t)count) {
-            a.kept[unit * a.keep + kept + at] = j;
-            a.to_weights[unit * a.keep + kept + at] = weight;
+        for (int i = 0; i < kSelectEach; ++i) {
+            const int j = j0 + i;
+            bool stay = j < length && (all || j < low || j >= high);
+            if (some && j >= low && j < high) stay = weight_key(own[i]) > prefix || (((same >> i) & 1u) && rank < need);
+            rank += (same >> i) & 1u;
+            if (stay) stays |= 1u << i;
         }
+        uint32_t at = kept + block_prefix((uint32_t)__builtin_popcount(stays), s_sums, &total);
         kept += total;
+        for (int i = 0; i < kSelectEach; ++i) {
+            if (((stays >> i) & 1u) && at < (uint32_t)count) {
+                a.kept[unit * a.keep + at] = j0 + i;
+                a.to_weights[unit * a.keep + at] = own[i];
+                ++at;
+            }
+        }
     }
     for (int i = count + tid; i < a.keep; i += kSelectThreads) {
         a.kept[unit * a.keep + i] = -1;
         a.to_weights[unit * a.keep + i] = 0.0f;
     }
+    if (h == 0 && tid == 0) a.to_lengths[s] = count;
 }
 
-// A wave moves the kept rows into one record of the new pages.
+// A wave moves the kept rows into one record of the new pages: where each comes from is found once and handed out through LDS.
 template <int NB>
 __global__ __launch_bounds__(256) void k_cache_move(EvictArgs a, int records)
 {
+    __shared__ uint64_t s_from[4][kRecordSlots];         // its record's place among the pages, all ones: none, which is moved as zeros
+    __shared__ int s_slot[4][kRecordSlots];              // its slot of that record
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const uint32_t groups = ((uint32_t)records + 3) / 4;
     const int it = (int)(blockIdx.x % groups) * 4 + wave;
     const int h = (int)(blockIdx.x / groups % (unsigned)a.c.kv_heads);
     const int s = (int)(blockIdx.x / groups / (unsigned)a.c.kv_heads);
     const int length = sequence_length(a.c, s), count = length < a.keep ? length : a.keep;
-    const int left = count - it * kRecordSlots;     // rows of this record
+    const int left = count - it * kRecordSlots < kRecordSlots ? count - it * kRecordSlots : kRecordSlots;     // rows of this record
     if (left <= 0) return;
     uint8_t *to = record_of(a.c, a.to_table, a.to_table_stride, s, h, it * kRecordSlots, NB);
     if (!to) return;
-    const int32_t *kept = a.kept + ((uint64_t)s * a.c.kv_heads + h) * a.keep + it * kRecordSlots;
-    // keys: 16 bytes of a row at a time
-    for (int u = lane; u < 32 * NB; u += 64) {
-        const int t = u / NB;
-        if (t >= left) continue;
-        const int slot = kept[t];
+    if (lane < left) {
+        const int slot = a.kept[((uint64_t)s * a.c.kv_heads + h) * a.keep + it * kRecordSlots + lane];
         const uint8_t *from = record_of(a.c, a.c.table, a.c.table_stride, s, h, slot, NB);
+        s_from[wave][lane] = from ? (uint64_t)(from - a.c.pages) : ~0ull;
+        s_slot[wave][lane] = slot & 31;
+    }
+    wave_lds_order();
+    // keys: 16 bytes of a row at a time
+    for (int u = lane; u < left * NB; u += 64) {
+        const int t = u / NB, slot = s_slot[wave][t];
+        const uint64_t place = s_from[wave][t];
+        const uint8_t *from = a.c.pages + place;
         u32x4 v = {0, 0, 0, 0};
-        if (from) v = *(const u32x4 *)(from + (slot & 31) * 16 * NB + (u % NB) * 16);
-        *(u32x4 *)(to + u * 16) = v;
         uint16_t lo = 0;
-        if (from) lo = *(const uint16_t *)(from + kKeyLows * NB + ((slot & 31) * NB + u % NB) * 2);
+        if (place != ~0ull) {
+            v = *(const u32x4 *)(from + slot * 16 * NB + (u % NB) * 16);
+            lo = *(const uint16_t *)(from + kKeyLows * NB + (slot * NB + u % NB) * 2);
+        }
+        *(u32x4 *)(to + u * 16) = v;
         *(uint16_t *)(to + kKeyLows * NB + u * 2) = lo;
     }
-    // what lies by eights of slots: values' codes (8 NB units of 16 bytes for every eight), steps and lowest numbers (NB units)
-    constexpr uint32_t kParts[4] = {kValueCodes, kKeySteps, kValueSteps, kValueLows};
-    for (int part = 0; part < 4; ++part) {
-        const int units = part == 0 ? 8 * NB : NB;
-        for (int u = lane; u < 4 * units; u += 64) {
-            const int octet = u / units, unit = u % units;
-            for (int e = 0; e < 8; ++e) {
-                const int t = octet * 8 + e;
-                if (t >= left) break;
-                const int slot = kept[t];
-                const uint8_t *from = record_of(a.c, a.c.table, a.c.table_stride, s, h, slot, NB);
-                uint16_t v = 0;
-                if (from) v = *(const uint16_t *)(from + kParts[part] * NB + ((((slot & 31) >> 3) * units) + unit) * 16 + (slot & 7) * 2);
-                *(uint16_t *)(to + kParts[part] * NB + u * 16 + e * 2) = v;
-            }
+    // what lies by eights of slots, in units of 16 bytes: values' codes (8 NB units for every eight), steps of both, values' lowest numbers (NB each)
+    for (int u = lane; u < 44 * NB; u += 64) {
+        const int octet = u / (11 * NB), place = u % (11 * NB);
+        const int part = place < 8 * NB ? 0 : 1 + (place - 8 * NB) / NB, units = part == 0 ? 8 * NB : NB;
+        const int unit = part == 0 ? place : (place - 8 * NB) % NB;
+        const uint32_t offset = (part == 0 ? kValueCodes : (part == 1 ? kKeySteps : (part == 2 ? kValueSteps : kValueLows))) * NB;
+        uint32_t word[8];
+        for (int e = 0; e < 8; ++e) {
+            const int t = octet * 8 + e, slot = t < left ? s_slot[wave][t] : 0;
+            const uint64_t from = t < left ? s_from[wave][t] : ~0ull;
+            word[e] = from != ~0ull ? *(const uint16_t *)(a.c.pages + from + offset + ((slot >> 3) * units + unit) * 16 + (slot & 7) * 2) : 0u;
+        }
+        uint8_t *at = to + offset + (octet * units + unit) * 16;
+        if (octet * 8 + 8 <= left) {
+            *(u32x4 *)at = u32x4{word[0] | (word[1] << 16), word[2] | (word[3] << 16), word[4] | (word[5] << 16), word[6] | (word[7] << 16)};
+        } else {
+            for (int e = 0; e < 8; ++e)
+                if (octet * 8 + e < left) ((uint16_t *)at)[e] = (uint16_t)word[e];
         }
     }
 }
@@ -1412,11 +1540,17 @@ __global__ __launch_bounds__(256) void k_cache_move(EvictArgs a, int records)
 template <bool STORE, int TY>
 static hipError_t rows_of_type(const CacheArgs &c, const RowsArgs &r, int nb, hipStream_t s)
 {
-    const uint64_t threads = (uint64_t)r.n_rows * (uint32_t)c.kv_heads * (uint32_t)nb * 4;
-    const dim3 grid((uint32_t)((threads + 255) / 256)), block(256);
-    if (nb == 2) hipLaunchKernelGGL((k_cache_rows<2, TY, STORE>), grid, block, 0, s, c, r);
-    else if (nb == 4) hipLaunchKernelGGL((k_cache_rows<4, TY, STORE>), grid, block, 0, s, c, r);
-    else hipLaunchKernelGGL((k_cache_rows<8, TY, STORE>), grid, block, 0, s, c, r);
+    const uint32_t items = ((uint32_t)r.n_rows / kRowsOfWave + 2u * (uint32_t)c.n_seqs) * (uint32_t)c.kv_heads;
+    const dim3 grid((items + 3) / 4), block(256);
+    if (STORE) {
+        if (nb == 2) hipLaunchKernelGGL((k_cache_store<2, TY>), grid, block, 0, s, c, r, items);
+        else if (nb == 4) hipLaunchKernelGGL((k_cache_store<4, TY>), grid, block, 0, s, c, r, items);
+        else hipLaunchKernelGGL((k_cache_store<8, TY>), grid, block, 0, s, c, r, items);
+    } else {
+        if (nb == 2) hipLaunchKernelGGL((k_cache_load<2, TY>), grid, block, 0, s, c, r, items);
+        else if (nb == 4) hipLaunchKernelGGL((k_cache_load<4, TY>), grid, block, 0, s, c, r, items);
+        else hipLaunchKernelGGL((k_cache_load<8, TY>), grid, block, 0, s, c, r, items);
+    }
     return hipGetLastError();
 }
 hipError_t launch_cache_store(const CacheArgs &c, const RowsArgs &r, int nb, int type, hipStream_t s)
