@@ -31,6 +31,7 @@ struct RowsArgs {
     uint64_t row_stride, head_stride;
     const int32_t *starts;
     int32_t n_rows;
+    int32_t aligned;            // every eight numbers lie at a multiple of 16 bytes
 };
 
 struct AttendArgs {
@@ -44,6 +45,7 @@ struct AttendArgs {
     int32_t tiles;              // column tiles a sequence's rows can take
     int32_t splits;             // parts the records are cut into, and
     int32_t split_records;      // records of a part, a multiple of kAttendWaves
+    int32_t q_aligned;          // every eight numbers of q lie at a multiple of 16 bytes
     int32_t causal, window;     // window 0: none
     float scale;
     float *lse;                 // null: not wanted

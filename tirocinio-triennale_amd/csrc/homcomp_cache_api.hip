@@ -23,6 +23,10 @@ int launched(hipError_t e)
 
 inline bool aligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 inline uintptr_t bytes_of(int type) { return type == HOMCOMP_F32 ? 4 : 2; }
+inline bool eights_aligned(const void *p, int type, size_t row_stride, size_t head_stride)
+{
+    return aligned(p, 16) && (row_stride | head_stride) % (16 / bytes_of(type)) == 0;
+}
 inline bool type_ok(int type) { return type == HOMCOMP_BF16 || type == HOMCOMP_F16 || type == HOMCOMP_F32; }
 
 // Blocks of a row, 0 where the shape is not supported.
@@ -79,7 +83,8 @@ int rows_call(bool store, const homcomp_cache *cache, void *k, void *v, int type
     if (!k || !v || !starts) return HOMCOMP_ERR_INVALID_ARG;
     if (!aligned(k, bytes_of(type)) || !aligned(v, bytes_of(type)) || !aligned(starts, 4)) return HOMCOMP_ERR_ALIGNMENT;
     if (!store && k == v) return HOMCOMP_ERR_INVALID_ARG;
-    const hc::RowsArgs r = {k, v, row_stride, head_stride, starts, (int32_t)n_rows};
+    const bool eights = eights_aligned(k, type, row_stride, head_stride) && aligned(v, 16);
+    const hc::RowsArgs r = {k, v, row_stride, head_stride, starts, (int32_t)n_rows, eights ? 1 : 0};
     return launched(store ? hc::launch_cache_store(c, r, nb, type, (hipStream_t)stream) : hc::launch_cache_load(c, r, nb, type, (hipStream_t)stream));
 }
 
@@ -200,6 +205,7 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t,
     a.tiles = p.tiles;
     a.splits = p.splits;
     a.split_records = p.split_records;
+    a.q_aligned = eights_aligned(t->d_q, t->type, t->q_row_stride, t->q_head_stride) ? 1 : 0;
     a.causal = t->causal ? 1 : 0;
     a.window = t->window > (size_t)kMostSlots ? 0 : (int32_t)t->window;   // (no slot is that far away)
     a.scale = t->scale;

@@ -23,37 +23,44 @@ __device__ __forceinline__ float f16_to_f32(uint32_t bits) { return (float)__bui
 __device__ __forceinline__ uint32_t f32_to_f16(float x) { return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x); }
 
 template <int TY>
-__device__ __forceinline__ float load_number(const void *base, uint64_t at)
-{
-    if (TY == kBf16) return bf16_to_f32(((const uint16_t *)base)[at]);
-    if (TY == kF16) return f16_to_f32(((const uint16_t *)base)[at]);
-    return ((const float *)base)[at];
-}
-template <int TY>
 __device__ __forceinline__ void store_number(void *base, uint64_t at, float x)
 {
     if (TY == kBf16) ((uint16_t *)base)[at] = (uint16_t)f32_to_bf16(x);
     else if (TY == kF16) ((uint16_t *)base)[at] = (uint16_t)f32_to_f16(x);
     else ((float *)base)[at] = x;
 }
-// Eight adjacent numbers; 16-byte accesses where the address allows them.
+// Eight adjacent numbers; `aligned`: all such addresses of the tensor are multiples of 16 bytes.  (The host says so: with a branch on each
+// address every load was waited for by itself, four times the latency in front of a wave's work.)
 template <int TY>
-__device__ __forceinline__ void load8(const void *base, uint64_t at, float *x)
+struct Eight {
+    u32x4 w[TY == kF32 ? 2 : 1];
+};
+template <int TY>
+__device__ __forceinline__ Eight<TY> load_eight(const void *base, uint64_t at, bool aligned)
 {
     const uint8_t *p = (const uint8_t *)base + at * (TY == kF32 ? 4 : 2);
-    if (((uintptr_t)p & 15u) == 0) {
-        if (TY == kF32) {
-            const f32x4 a = *(const f32x4 *)p, b = *(const f32x4 *)(p + 16);
-            for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-        } else {
-            const u32x4 w = *(const u32x4 *)p;
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t bits = (w[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-                x[i] = TY == kBf16 ? bf16_to_f32(bits) : f16_to_f32(bits);
-            }
-        }
+    Eight<TY> r;
+    if (aligned) {
+        r.w[0] = *(const u32x4 *)p;
+        if (TY == kF32) r.w[sizeof r.w / 16 - 1] = *(const u32x4 *)(p + 16);
+    } else if (TY == kF32) {
+        for (int i = 0; i < 8; ++i) r.w[(i >> 2) % (sizeof r.w / 16)][i & 3] = ((const uint32_t *)p)[i];
     } else {
-        for (int i = 0; i < 8; ++i) x[i] = load_number<TY>(base, at + (uint64_t)i);
+        for (int i = 0; i < 4; ++i) r.w[0][i] = (uint32_t)((const uint16_t *)p)[2 * i] | ((uint32_t)((const uint16_t *)p)[2 * i + 1] << 16);
+    }
+    return r;
+}
+template <int TY>
+__device__ __forceinline__ void numbers_of(const Eight<TY> &r, float *x)
+{
+    for (int i = 0; i < 8; ++i) {
+        if (TY == kF32) {
+            const uint32_t bits = r.w[(i >> 2) % (sizeof r.w / 16)][i & 3];
+            x[i] = __builtin_bit_cast(float, bits);
+        } else {
+            const uint32_t bits = (r.w[0][i >> 1] >> (16 * (i & 1))) & 0xffffu;
+            x[i] = TY == kBf16 ? bf16_to_f32(bits) : f16_to_f32(bits);
+        }
     }
 }
 template <int TY>
@@ -231,17 +238,20 @@ struct RowsItem {
     int begin, end;     // slots of it that are rows: slot0 + begin .. slot0 + end - 1
     int row0;           // packed row of slot0 (may be in front of the first)
 };
-__device__ __forceinline__ RowsItem rows_item(const CacheArgs &c, const RowsArgs &a, uint32_t item)
+__device__ __forceinline__ RowsItem rows_item(const CacheArgs &c, const RowsArgs &a, uint32_t item, int lane)
 {
     RowsItem r = {-1, (int)(item % (uint32_t)c.kv_heads), 0, 0, 0, 0};
     const int v = (int)(item / (uint32_t)c.kv_heads);
-    int lo = 0, hi = c.n_seqs;   // the last s with base(s) <= v
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        int at = a.starts[mid];
+    // the last sequence whose first item is at or in front of v: 64 of them looked at together
+    int lo = 0;
+    for (int n = c.n_seqs; n > 1;) {
+        const int step = (n + 63) >> 6, own = lo + lane * step;
+        int at = lane * step < n ? a.starts[own] : 0;
         at = at < 0 ? 0 : (at > a.n_rows ? a.n_rows : at);
-        if ((at >> 4) + 2 * mid <= v) lo = mid;
-        else hi = mid;
+        const int m = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane * step < n && (at >> 4) + 2 * own <= v));
+        const int skip = m > 0 ? (m - 1) * step : 0;
+        lo += skip;
+        n = n - skip < step ? n - skip : step;
     }
     const Rows rows = rows_of(a.starts, lo, a.n_rows);
     const int first = rows.first, count = rows.count, length = sequence_length(c, lo);
@@ -274,20 +284,29 @@ __global__ __launch_bounds__(256) void k_cache_store(CacheArgs c, RowsArgs a, ui
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const uint32_t item = blockIdx.x * 4u + (uint32_t)wave;
     if (item >= items) return;
-    const RowsItem r = rows_item(c, a, item);
+    const RowsItem r = rows_item(c, a, item, lane);
     if (r.s < 0) return;
     uint8_t *rec = record_of(c, c.table, c.table_stride, r.s, r.h, r.slot0, NB);
     if (!rec) return;
     const int t = lane >> 2, j = lane & 3, slot = (r.slot0 & 31) + t;   // slot of the record
     const bool own = t >= r.begin && t < r.end;
     const uint64_t at = (uint64_t)(int64_t)(r.row0 + (own ? t : r.begin)) * a.row_stride + (uint64_t)r.h * a.head_stride + (uint64_t)(8 * j);
-    float x[NB][8];
-    for (int b = 0; b < NB; ++b) load8<TY>(a.k, at + (uint64_t)(32 * b), x[b]);
+    Eight<TY> keys[NB], values[NB];
+    if (a.aligned) {
+        for (int b = 0; b < NB; ++b) keys[b] = load_eight<TY>(a.k, at + (uint64_t)(32 * b), true);
+        for (int b = 0; b < NB; ++b) values[b] = load_eight<TY>(a.v, at + (uint64_t)(32 * b), true);
+    } else {
+        for (int b = 0; b < NB; ++b) keys[b] = load_eight<TY>(a.k, at + (uint64_t)(32 * b), false);
+        for (int b = 0; b < NB; ++b) values[b] = load_eight<TY>(a.v, at + (uint64_t)(32 * b), false);
+    }
+    float x[8];
 #pragma unroll
     for (int half = 0; half < (NB + 3) / 4; ++half) {
         uint32_t w[4] = {0, 0, 0, 0}, step = 0, low = 0;
+#pragma unroll
         for (int n = 0; n < 4 && 4 * half + n < NB; ++n) {
-            const Block8 q = quantise(x[4 * half + n]);
+            numbers_of<TY>(keys[4 * half + n], x);
+            const Block8 q = quantise(x);
             for (int i = 0; i < 8; ++i) w[n] |= q.code[i] << (4 * (i >> 1) + 16 * (i & 1));
             if (j == n) step = q.s, low = q.lo;
         }
@@ -301,13 +320,14 @@ __global__ __launch_bounds__(256) void k_cache_store(CacheArgs c, RowsArgs a, ui
             }
         }
     }
-    for (int b = 0; b < NB; ++b) load8<TY>(a.v, at + (uint64_t)(32 * b), x[b]);
     uint32_t step[(NB + 3) / 4], low[(NB + 3) / 4];
 #pragma unroll
     for (int i = 0; i < NB / 2; ++i) {
         uint32_t word[4] = {0, 0, 0, 0};   // of units 16 i + 8 (j & 1) + 4 (j >> 1) + n
+#pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const Block8 q = quantise(x[2 * i + e]);
+            numbers_of<TY>(values[2 * i + e], x);
+            const Block8 q = quantise(x);
             // value m and value 16 + m of the block share a byte: lanes j and j ^ 2 exchange
             for (int n = 0; n < 4; ++n) {
                 const uint32_t give = j < 2 ? q.code[4 + n] : q.code[n];
@@ -350,7 +370,7 @@ __global__ __launch_bounds__(256) void k_cache_load(CacheArgs c, RowsArgs a, uin
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const uint32_t item = blockIdx.x * 4u + (uint32_t)wave;
     if (item >= items) return;
-    const RowsItem r = rows_item(c, a, item);
+    const RowsItem r = rows_item(c, a, item, lane);
     if (r.s < 0) return;
     const uint8_t *rec = record_of(c, c.table, c.table_stride, r.s, r.h, r.slot0, NB);
     const int t = lane >> 2, j = lane & 3, slot = (r.slot0 & 31) + t;
@@ -473,13 +493,22 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
     constexpr int NQ = query_parts<TY>();
     const bool there = column < count * a.group;
     const int row = there ? column / a.group : 0, head = there ? column - row * a.group : 0;
+    // (a column that is not there reads row 0 of the sequence, which is, and counts as zeros)
+    const uint64_t at = (uint64_t)(first + row) * a.q_row_stride + (uint64_t)(h * a.group + head) * a.q_head_stride + (uint64_t)(8 * g);
+    Eight<TY> raw[NB];
+    if (a.q_aligned) {
+        for (int b = 0; b < NB; ++b) raw[b] = load_eight<TY>(a.q, at + (uint64_t)(32 * b), true);
+    } else {
+        for (int b = 0; b < NB; ++b) raw[b] = load_eight<TY>(a.q, at + (uint64_t)(32 * b), false);
+    }
     float x[NB][8];
     float top = 0.0f;
     for (int b = 0; b < NB; ++b) {
-        for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
-        if (there)
-            load8<TY>(a.q, (uint64_t)(first + row) * a.q_row_stride + (uint64_t)(h * a.group + head) * a.q_head_stride + (uint64_t)(32 * b + 8 * g), x[b]);
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[b][i]));
+        numbers_of<TY>(raw[b], x[b]);
+        for (int i = 0; i < 8; ++i) {
+            x[b][i] = there ? x[b][i] : 0.0f;
+            top = fmaxf(top, fabsf(x[b][i]));
+        }
     }
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -510,9 +539,9 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
     const bf16x8 none = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
     r.sums = g == 0 ? parts[0] : (g == 1 ? parts[1] : (g == 2 ? parts[2] : none));
     r.factor = ldexpf(a.scale * kLog2e, (FORM == kWhole ? -14 : 10) + e);
-    const int at = slot0 + row;
-    r.see_to = !there ? 0 : (a.causal ? (at + 1 < length ? at + 1 : length) : length);
-    r.see_from = a.window > 0 && at + 1 - a.window > 0 ? at + 1 - a.window : 0;
+    const int own = slot0 + row;
+    r.see_to = !there ? 0 : (a.causal ? (own + 1 < length ? own + 1 : length) : length);
+    r.see_from = a.window > 0 && own + 1 - a.window > 0 ? own + 1 - a.window : 0;
 }
 
 // What a lane holds of a record: rows of the products' operands, and the scales of what it gets back.
