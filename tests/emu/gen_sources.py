@@ -159,8 +159,8 @@ CACHE_LIBRARY = os.path.join(GEN, "libhomcomp_cache_emu.so")
 CACHE_EDITS = [
     ('#include "homcomp_cache.hpp"', '#include "cache_emu.hpp"\n#include "homcomp_cache.hpp"\nthread_local emu_operands emu_products;'),
     ("{ return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)x); }", "{ return emu_f32_to_bf16(x); }"),
-    ('asm volatile("" : "+v"(zero));', "", 2),
-    ('asm volatile("" : "+v"(from));', "", 3),
+    ('asm volatile("" : "+v"(zero));', ""),
+    ('asm volatile("" : "+v"(x));', ""),
     ("{ return __builtin_elementwise_fma(a, b, c); }",
      "{ return f16x2{(_Float16)fmaf((float)a[0], (float)b[0], (float)c[0]), (_Float16)fmaf((float)a[1], (float)b[1], (float)c[1])}; }"),
     ("{ return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b}); }", "{ return emu_f32_to_bf16(a) | (emu_f32_to_bf16(b) << 16); }"),

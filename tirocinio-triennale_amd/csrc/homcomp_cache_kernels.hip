@@ -448,8 +448,6 @@ constexpr float kNegInf = -INFINITY;
 
 template <int TY>
 constexpr int query_parts() { return TY == kF32 ? 3 : 1; }
-template <int TY>
-constexpr int weight_parts() { return TY == kF32 ? 3 : 2; }
 
 template <int NB, int NQ>
 struct Queries {
@@ -697,64 +695,58 @@ __device__ __forceinline__ void write_result(const AttendArgs &a, int h, int fir
             total == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
+// Values the compiler is not to look through: a register of zeros for products to start from (it would clear one for each), a number that
+// comparisons under a rare branch depend on (it would make them in front of the branch).
+__device__ __forceinline__ f32x4 kept_zero()
+{
+    f32x4 zero = {0, 0, 0, 0};
+    asm volatile("" : "+v"(zero));
+    return zero;
+}
+__device__ __forceinline__ int kept_here(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// Two codes as float16 numbers: at bits 0 .. 3 under 1024, at bits 4 .. 7 under 64, both exact.
+// (The numbers they stand under are held in registers: one instruction then joins and masks.)
+struct Under {
+    uint32_t of_0, of_4;
+};
+__device__ __forceinline__ Under under_codes() { return {(uint32_t)kept_here(0x64006400), (uint32_t)kept_here(0x54005400)}; }
+__device__ __forceinline__ f16x2 codes_at_0(uint32_t w, const Under &u) { return __builtin_bit_cast(f16x2, (w & 0x000f000fu) | u.of_0) - (_Float16)1024.0f; }
+__device__ __forceinline__ f16x2 codes_at_4(uint32_t w, const Under &u) { return __builtin_bit_cast(f16x2, (w & 0x00f000f0u) | u.of_4) - (_Float16)64.0f; }
+__device__ __forceinline__ f16x2 fma_pair(f16x2 a, f16x2 b, f16x2 c) { return __builtin_elementwise_fma(a, b, c); }
+
+// Whether a block is for float16: s from 2^-13 to 2^11 and lo up to 2^15 in size; where s is 0, lo 0 or from 2^-13.
+__device__ __forceinline__ bool for_float16(uint32_t s, uint32_t lo)
+{
+    lo &= 0x7fffu;
+    return s <= 0x6800u && lo <= 0x4700u && (s >= 0x0800u || (s == 0 && (lo == 0 || lo >= 0x3900u)));
+}
 // What a wave has gathered for its columns.
 template <int NB>
 struct Gathered {
-    f32x4 o[NB / 2][4];   // sum of (code - 8 or 7) * p s_b, values 64 i + 16 p + 4 g + r, times 2^-69 (2^-65 where codes stand higher)
-    f32x4 low;            // what block 4 g + r adds to all its values, times 2^64
+    f32x4 o[NB / 2][4];   // sum of value * p, values 64 i + 16 p + 4 g + r, times 2^7
     float top;            // exponent p is relative to; at most 8 below the largest so far
-    float total;          // sum of the lane's p, times 2^64
+    float total;          // sum of the lane's p, times 2^7
 };
 
-// One record.  A new reference exponent costs a multiplication of everything gathered, so it is taken only where a weight
-// would exceed 2^8 (32-bit sums have room for that); a lane looks at its own eight slots alone, and lanes exchange only then.
-template <int NB, int NQ, int NP, bool FINE>
-__device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<NB, NQ> &q, int lane, int slot0, int length, bool masked, const f32x4 &zero, Gathered<NB> &s)
+// The values' product in exact codes, for any values: p s_b in NP parts of bfloat16 against the codes.
+// Codes count from the middle, c - 8 in even slots and c - 7 in odd ones (numbers of the codes' own form; on the average the
+// middle itself), the rest is lo + 8 s or lo + 7 s: with codes from 0 the two sums would grow with the number of slots and nearly
+// cancel where a block's values lie around zero, each with roundings of its own.
+template <int NB, int NQ, int NP>
+__device__ __forceinline__ void values_by_codes(const uint8_t *at, const Queries<NB, NQ> &q, int lane, int slot0, int length, bool masked, const f32x4 &zero,
+                                                float (&p)[8], Gathered<NB> &s)
 {
-    f32x4 x[2];
-    KeyPart<NB> k;
-    take_keys<NB>(at, lane, k);
-    record_scores<NB, NQ, FINE>(k, q, zero, x);
+    constexpr bool kFineValues = NP == 3;
+    const int n16 = lane & 15;
     ValuePart<NB> v;
     take_values<NB>(at, lane, v);
-    // 2^64 goes in with the exponent, except for 32-bit results: next to 64 an exponent keeps 2^-19, too little for them
-    constexpr float kUp = NP == 3 ? 0.0f : 64.0f;
-    float e[8], most = kNegInf;
-    const float bias = kUp - s.top;      // (nothing seen yet: +infinity, which asks for a reference)
-    for (int i = 0; i < 8; ++i) e[i] = fmaf(x[i >> 2][i & 3], q.factor, bias);
-    if (masked) {
-        int from = slot0;
-        asm volatile("" : "+v"(from));   // (the comparisons stay under the branch)
-        for (int i = 0; i < 8; ++i) e[i] = sees(q, from + i) ? e[i] : kNegInf;
-    }
-    for (int i = 0; i < 8; ++i) most = fmaxf(most, e[i]);
-    if (__builtin_amdgcn_ballot_w64(most > kUp + 8.0f) != 0) {
-        most = kNegInf;
-        for (int i = 0; i < 8; ++i)
-            if (!masked || sees(q, slot0 + i)) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
-        most = fmaxf(most, __shfl_xor(most, 16, 64));
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const float now = fmaxf(s.top, most);
-        const float shrink = now == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(s.top - now);   // (nothing so far: 0)
-        s.top = now;
-        s.total *= shrink;
-        for (int r = 0; r < 4; ++r) {
-            s.low[r] *= shrink;
-            for (int i = 0; i < NB / 2; ++i)
-                for (int n = 0; n < 4; ++n) s.o[i][n][r] *= shrink;
-        }
-        for (int i = 0; i < 8; ++i) e[i] = !masked || sees(q, slot0 + i) ? fmaf(x[i >> 2][i & 3], q.factor, kUp - now) : kNegInf;
-    }
-    float p[8];
-    for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(e[i]);
-        if (NP == 3) p[i] *= 0x1p64f;
-        s.total += p[i];
-    }
-    // Codes count from the middle, c - 8 in even slots and c - 7 in odd ones (numbers of the codes' own form; on the average the
-    // middle itself), the rest is lo + 8 s or lo + 7 s: with codes from 0 the two sums would grow with the number of slots and nearly
-    // cancel where a block's values lie around zero, each with roundings of its own.
-    u32x4 middle[NP];
+    for (int i = 0; i < 8; ++i) p[i] *= 0x1p57f;   // 2^64 with the 2^7 they have: products with codes of 2^-133 stay normal numbers
+    bf16x8 w[NP], middle[NP];
     {
         float mid[8];
         for (int i = 0; i < 8; ++i) {
@@ -765,45 +757,127 @@ __device__ __forceinline__ void attend_record(const uint8_t *at, const Queries<N
         if (masked)
             for (int i = 0; i < 8; ++i)
                 if (slot0 + i >= length || !(mid[i] == mid[i])) mid[i] = 0.0f;
-        bf16x8 parts[NP];
-        split_bf16<NP>(mid, parts);
-        for (int n = 0; n < NP; ++n) middle[n] = __builtin_bit_cast(u32x4, parts[n]);
+        split_bf16<NP>(mid, middle);
     }
-    bf16x8 w[NP];
     split_bf16<NP>(p, w);
+    f32x4 low = zero;   // what block 4 g + r adds to all its values, times 2^64
     for (int n = 0; n < NP; ++n)
-        for (int e2 = 0; n + e2 < NP; ++e2)
-            s.low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, middle[n]), w[e2], s.low, 0, 0, 0);
+        for (int e = 0; n + e < NP; ++e) low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle[n], w[e], low, 0, 0, 0);
     for (int b = 0; b < NB; ++b) {
         float ps[8];
         for (int i = 0; i < 8; ++i) ps[i] = fmaf((float)v.steps[b][i], p[i], 0.0f);
         if (masked) {
-            int from = slot0;
-            asm volatile("" : "+v"(from));
+            const int from = kept_here(slot0);
             for (int i = 0; i < 8; ++i) ps[i] = sees(q, from + i) ? ps[i] : 0.0f;
         }
         split_bf16<NP>(ps, w);
         const u32x4 codes = v.codes[b >> 1];
-        constexpr bool kFineValues = NP == 3;
+        const float base = __shfl(low[b & 3], n16 + 16 * (b >> 2), 64) * 0x1p-57f;
         for (int n = 0; n < 2; ++n) {
             u32x4 c;
             for (int i = 0; i < 4; ++i) c[i] = code_pairs<kFineValues>(codes[i])[2 * (b & 1) + n];
             const uint32_t back = kFineValues || n ? 0x80708080u : 0x80078008u;
-            f32x4 &o = s.o[b >> 1][2 * (b & 1) + n];
-            for (int e2 = 0; e2 < NP; ++e2) {
-                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), w[e2], o, 0, 0, 0);
-                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{back, back, back, back}), w[e2], o, 0, 0, 0);
+            f32x4 o = zero;   // times 2^-69, 2^-65 where codes stand higher
+            for (int e = 0; e < NP; ++e) {
+                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), w[e], o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{back, back, back, back}), w[e], o, 0, 0, 0);
             }
+            for (int r = 0; r < 4; ++r) s.o[b >> 1][2 * (b & 1) + n][r] += fmaf(o[r], kFineValues || n ? 0x1p72f : 0x1p76f, base);
         }
     }
+}
+
+// Values as float16 numbers, where all of a record's blocks are for float16 (for 16-bit results): p in one part, two for float16 results.
+// A third of the vector instructions of the product in codes, and no more off than the results' own rounding.
+template <int NB, int NP>
+__device__ __forceinline__ void values_by_numbers(const uint8_t *at, const uint8_t *lows, const Under &under, int lane, const float (&p)[8], Gathered<NB> &s)
+{
+    const int m = lane & 15, g = lane >> 4;
+    f16x8 w[NP];
+    for (int i = 0; i < 8; ++i) {
+        w[0][i] = (_Float16)p[i];
+        if (NP == 2) w[NP - 1][i] = (_Float16)(p[i] - (float)w[0][i]);
+    }
+    for (int b = 0; b < NB; ++b) {
+        const u32x4 codes = *(const u32x4 *)(at + kValueCodes * NB + g * 128 * NB + ((b >> 1) * 16 + m) * 16);
+        const u32x4 step = *(const u32x4 *)(at + kValueSteps * NB + (g * NB + b) * 16), low = *(const u32x4 *)(lows + (g * NB + b) * 16);
+        for (int n = 0; n < 2; ++n) {
+            u32x4 v;
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t word = (b & 1) ? codes[i] >> 8 : codes[i], sw = step[i], lw = low[i];   // (a cast of an element in place takes the vector's first one)
+                v[i] = __builtin_bit_cast(uint32_t, fma_pair(n ? codes_at_4(word, under) : codes_at_0(word, under), __builtin_bit_cast(f16x2, sw), __builtin_bit_cast(f16x2, lw)));
+            }
+            f32x4 &o = s.o[b >> 1][2 * (b & 1) + n];
+            for (int e = 0; e < NP; ++e) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v), w[e], o, 0, 0, 0);
+        }
+    }
+}
+
+// One record.  A new reference exponent costs a multiplication of everything gathered, so it is taken only where a weight
+// would exceed 2^8 (32-bit sums have room for that); a lane looks at its own eight slots alone, and lanes exchange only then.
+template <int NB, int TY, bool FINE>
+__device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, query_parts<TY>()> &q, int lane, int slot0, int length, bool masked, const f32x4 &zero, const Under &under, Gathered<NB> &s)
+{
+    constexpr int NQ = query_parts<TY>();
+    f32x4 x[2];
+    {
+        KeyPart<NB> k;
+        take_keys<NB>(at, lane, k);
+        record_scores<NB, NQ, FINE>(k, q, zero, x);
+    }
+    // Values for float16?  The lanes look at the blocks together, and leave the lowest numbers as float16 behind the record.
+    bool numbers = false;
+    if (TY != kF32 && !masked) {
+        bool fine = true;
+        for (int i = 0; i < (NB + 3) / 4; ++i) {
+            const int pair = 64 * i + lane;
+            if (pair < 16 * NB) {
+                const uint32_t step = *(const uint32_t *)(at + kValueSteps * NB + pair * 4), low = *(const uint32_t *)(at + kValueLows * NB + pair * 4);
+                fine = fine && for_float16(step & 0xffffu, low & 0xffffu) && for_float16(step >> 16, low >> 16);
+                const f16x2 l = {(_Float16)bf16_to_f32(low & 0xffffu), (_Float16)__builtin_bit_cast(float, low & 0xffff0000u)};
+                *(uint32_t *)(at + record_bytes(NB) + pair * 4) = __builtin_bit_cast(uint32_t, l);
+            }
+        }
+        numbers = __builtin_amdgcn_ballot_w64(!fine) == 0;
+        wave_lds_order();
+    }
+    float p[8], most = kNegInf;
+    const float bias = 7.0f - s.top;      // (nothing seen yet: +infinity, which asks for a reference)
+    for (int i = 0; i < 8; ++i) p[i] = fmaf(x[i >> 2][i & 3], q.factor, bias);
+    if (masked) {
+        const int from = kept_here(slot0);
+        for (int i = 0; i < 8; ++i) p[i] = sees(q, from + i) ? p[i] : kNegInf;
+    }
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
+    if (__builtin_amdgcn_ballot_w64(most > 15.0f) != 0) {
+        most = kNegInf;
+        for (int i = 0; i < 8; ++i)
+            if (!masked || sees(q, slot0 + i)) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const float now = fmaxf(s.top, most);
+        const float shrink = now == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(s.top - now);   // (nothing so far: 0)
+        s.top = now;
+        s.total *= shrink;
+        for (int r = 0; r < 4; ++r)
+            for (int i = 0; i < NB / 2; ++i)
+                for (int n = 0; n < 4; ++n) s.o[i][n][r] *= shrink;
+        for (int i = 0; i < 8; ++i) p[i] = !masked || sees(q, slot0 + i) ? fmaf(x[i >> 2][i & 3], q.factor, 7.0f - now) : kNegInf;
+    }
+    for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(p[i]);
+        s.total += p[i];
+    }
+    if (TY != kF32 && numbers) values_by_numbers<NB, TY == kF16 ? 2 : 1>(at, at + record_bytes(NB), under, lane, p, s);
+    else values_by_codes<NB, NQ, TY == kF32 ? 3 : 2>(at, q, lane, slot0, length, masked, zero, p, s);
 }
 
 template <int NB, int TY, bool FINE>
 __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) void k_cache_attend(AttendArgs a)
 {
-    constexpr int NQ = query_parts<TY>(), NP = weight_parts<TY>(), D = 32 * NB;
+    constexpr int NQ = query_parts<TY>(), D = 32 * NB;
     // the waves' records on their way, and afterwards their results
-    constexpr int kMem = kAttendWaves * (kColumns * (D + 4) * 4 > (int)record_bytes(NB) ? kColumns * (D + 4) * 4 : (int)record_bytes(NB));
+    constexpr int kStage = (int)record_bytes(NB) + 64 * NB, kMem = kAttendWaves * (kColumns * (D + 4) * 4 > kStage ? kColumns * (D + 4) * 4 : kStage);
     __shared__ __align__(16) uint8_t s_mem[kMem];
     float (*s_o)[kColumns][D + 4] = (float (*)[kColumns][D + 4])s_mem;
     __shared__ float s_top[kAttendWaves][kColumns], s_total[kAttendWaves][kColumns];
@@ -831,14 +905,13 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     Queries<NB, NQ> q;
     load_queries<NB, TY, FINE ? kFine : kLow>(a, h, first, count, slot0, length, tile * kColumns + n, g, q);
     Gathered<NB> acc;
-    acc.low = f32x4{0, 0, 0, 0};
     for (int i = 0; i < NB / 2; ++i)
         for (int p = 0; p < 4; ++p) acc.o[i][p] = f32x4{0, 0, 0, 0};
     acc.top = kNegInf;
     acc.total = 0.0f;
-    uint8_t *stage = s_mem + wave * (int)record_bytes(NB);
-    f32x4 zero = {0, 0, 0, 0};
-    asm volatile("" : "+v"(zero));   // a register of zeros for the products to start from, instead of one cleared for each
+    uint8_t *stage = s_mem + wave * kStage;
+    const f32x4 zero = kept_zero();
+    const Under under = under_codes();
     RawRecord<NB> raw;
     int it = from + wave;
     PagesAhead pages = {0, it, kAttendWaves, to};
@@ -850,8 +923,8 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
         if (rec) lay_record<NB>(stage, lane, raw);
         if (next_rec) load_record<NB>(next_rec, lane, raw);
         if (rec) {
-            attend_record<NB, NQ, NP, FINE>(stage, q, lane, it * kRecordSlots + 8 * g, length,
-                                            it * kRecordSlots < all_from || (it + 1) * kRecordSlots > all_to, zero, acc);
+            attend_record<NB, TY, FINE>(stage, q, lane, it * kRecordSlots + 8 * g, length,
+                                        it * kRecordSlots < all_from || (it + 1) * kRecordSlots > all_to, zero, under, acc);
         }
         it = next;
         rec = next_rec;
@@ -865,14 +938,12 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     total += __shfl_xor(total, 32, 64);
     if (g == 0) {
         s_top[wave][n] = top;
-        s_total[wave][n] = total * 0x1p-64f;
+        s_total[wave][n] = total * 0x1p-7f;
     }
     for (int i = 0; i < NB / 2; ++i) {
         for (int p = 0; p < 4; ++p) {
-            const int b = 2 * i + (p >> 1);
             f32x4 v;
-            const float base = __shfl(acc.low[b & 3], n + 16 * (b >> 2), 64) * 0x1p-64f;
-            for (int r = 0; r < 4; ++r) v[r] = fmaf(acc.o[i][p][r], NP == 3 || (p & 1) ? 0x1p65f : 0x1p69f, base);
+            for (int r = 0; r < 4; ++r) v[r] = acc.o[i][p][r] * 0x1p-7f;
             *(f32x4 *)&s_o[wave][n][64 * i + 16 * p + 4 * g] = v;
         }
     }
@@ -937,27 +1008,15 @@ __device__ __forceinline__ u32x4 load_unit(const uint8_t *rec, int unit, int lan
     }
     return codes;
 }
-// Two codes as float16 numbers: at bits 0 .. 3 under 1024, at bits 4 .. 7 under 64, both exact.
-__device__ __forceinline__ f16x2 codes_at_0(uint32_t w) { return __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u) - (_Float16)1024.0f; }
-__device__ __forceinline__ f16x2 codes_at_4(uint32_t w) { return __builtin_bit_cast(f16x2, (w & 0x00f000f0u) | 0x54005400u) - (_Float16)64.0f; }
-
-__device__ __forceinline__ f16x2 fma_pair(f16x2 a, f16x2 b, f16x2 c) { return __builtin_elementwise_fma(a, b, c); }
-
 // Halves of a word that belong to slots in front of `left`: slots 8 g + 2 n and 8 g + 2 n + 1.
 __device__ __forceinline__ uint32_t held_halves(int g, int n, int left)
 {
     return (8 * g + 2 * n < left ? 0x0000ffffu : 0u) | (8 * g + 2 * n + 1 < left ? 0xffff0000u : 0u);
 }
-// Whether a block is for float16: s from 2^-13 to 2^11 and lo up to 2^15 in size; where s is 0, lo 0 or from 2^-13.
-__device__ __forceinline__ bool for_float16(uint32_t s, uint32_t lo)
-{
-    lo &= 0x7fffu;
-    return s <= 0x6800u && lo <= 0x4700u && (s >= 0x0800u || (s == 0 && (lo == 0 || lo >= 0x3900u)));
-}
 // Lays a unit into `at`; sides: the record's; left: slots of the record that the sequence holds (what lies behind counts for nothing).
 // False where a key's block is not for float16.
 template <int NB>
-__device__ __forceinline__ bool lay_unit(uint8_t *at, const uint8_t *sides, int unit, int lane, const u32x4 &codes, int left)
+__device__ __forceinline__ bool lay_unit(uint8_t *at, const uint8_t *sides, const Under &under, int unit, int lane, const u32x4 &codes, int left)
 {
     const int m = lane & 15, g = lane >> 4;
     if (unit < NB) {
@@ -969,7 +1028,7 @@ __device__ __forceinline__ bool lay_unit(uint8_t *at, const uint8_t *sides, int 
             const uint32_t w = codes[n], high = w >> 8;
             const float s = f16_to_f32(step), lo = n ? __builtin_bit_cast(float, lows & 0xffff0000u) : bf16_to_f32(lows & 0xffffu);
             fine = fine && for_float16(step, (lows >> (16 * n)) & 0xffffu);
-            const f16x2 c[4] = {codes_at_0(w), codes_at_4(w), codes_at_0(high), codes_at_4(high)};
+            const f16x2 c[4] = {codes_at_0(w, under), codes_at_4(w, under), codes_at_0(high, under), codes_at_4(high, under)};
             u32x4 first, rest;
             for (int i = 0; i < 4; ++i) {
                 const float x = fmaf((float)c[i][0], s, lo), y = fmaf((float)c[i][1], s, lo);
@@ -999,8 +1058,8 @@ __device__ __forceinline__ bool lay_unit(uint8_t *at, const uint8_t *sides, int 
         const f16x2 s = __builtin_bit_cast(f16x2, pair);
         const f16x2 lo = {(_Float16)bf16_to_f32(lows[n] & 0xffffu), (_Float16)__builtin_bit_cast(float, lows[n] & 0xffff0000u)};
         const uint32_t w = half ? codes[n] >> 8 : codes[n];
-        out[0][n] = __builtin_bit_cast(uint32_t, fma_pair(codes_at_0(w), s, lo));
-        out[1][n] = __builtin_bit_cast(uint32_t, fma_pair(codes_at_4(w), s, lo));
+        out[0][n] = __builtin_bit_cast(uint32_t, fma_pair(codes_at_0(w, under), s, lo));
+        out[1][n] = __builtin_bit_cast(uint32_t, fma_pair(codes_at_4(w, under), s, lo));
     }
     for (int n = 0; n < 2; ++n) *(u32x4 *)(at + WideRecord<NB>::kValues + ((i * 4 + 2 * half + n) * 64 + lane) * 16) = out[n];
     return true;
@@ -1031,8 +1090,7 @@ __device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB,
     for (int t = 0; t < CT; ++t) {
         for (int i = 0; i < 8; ++i) e[t][i >> 2][i & 3] *= q[t].factor;
         if (masked) {
-            int from = slot0;
-            asm volatile("" : "+v"(from));   // (the comparisons stay under the branch)
+            const int from = kept_here(slot0);
             for (int i = 0; i < 8; ++i) e[t][i >> 2][i & 3] = sees(q[t], from + i) ? e[t][i >> 2][i & 3] : kNegInf;
         }
         float most = kNegInf;
@@ -1144,11 +1202,12 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
         }
     };
     bool fine = true;
+    const Under under = under_codes();
     auto lay_codes = [&](int j, const Pair &p) __attribute__((always_inline)) {
         for (int k = 0; k < kUnits; ++k) {
             const int u = wave + k * W, r = u / (2 * NB);
             if (u < 2 * kPer * NB && p[r])
-                fine = lay_unit<NB>(s_mem[j & 1][r], s_sides[j & 1][r], (u + r * NB) % (2 * NB), lane, raw[k], length - (from + kPer * j + r) * kRecordSlots) && fine;
+                fine = lay_unit<NB>(s_mem[j & 1][r], s_sides[j & 1][r], under, (u + r * NB) % (2 * NB), lane, raw[k], length - (from + kPer * j + r) * kRecordSlots) && fine;
         }
         // the values' blocks, one a thread
         for (int k = 0; k < (32 * kPer * NB + 64 * W - 1) / (64 * W); ++k) {
@@ -1158,8 +1217,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
                                            *(const uint16_t *)&s_sides[j & 1][r][WideRecord<NB>::kVLows + block * 2]);
         }
     };
-    f32x4 zero = {0, 0, 0, 0};
-    asm volatile("" : "+v"(zero));   // a register of zeros for the products to start from, instead of one cleared for each
+    const f32x4 zero = kept_zero();
     Pair now = find(0), next = find(1), later = find(2);
     load_sides(now);
     load_codes(now);
