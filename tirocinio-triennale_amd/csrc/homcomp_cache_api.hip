@@ -118,9 +118,10 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
         p->wide_tiles = (p->tiles + p->tiles_in_wide - 1) / p->tiles_in_wide;
     }
     const int64_t groups = p->wide_tiles ? (int64_t)c->n_seqs * c->kv_heads * p->wide_tiles : units;   // workgroups without parts
-    // eight workgroups for every compute unit, so that sequences of different lengths even out, but eight records at least for
-    // every wave (and two where there is little in all)
-    int64_t splits = groups ? ((p->wide_tiles ? 2 : 8) * kComputeUnits + groups - 1) / groups : 1;
+    // eight workgroups for every compute unit, so that sequences of different lengths even out (a single one has nothing to even out: the two
+    // that a unit holds at once), but eight records at least for every wave (and two where there is little in all).
+    // 64 sequences of up to 8192 slots, 8 heads: 95 us with eight, 98 with four, 102 with two; one of 131072: 49 with eight or four, 43 with two.
+    int64_t splits = groups ? ((p->wide_tiles || c->n_seqs == 1 ? 2 : 8) * kComputeUnits + groups - 1) / groups : 1;
     const int64_t least = groups * records >= 64 * kComputeUnits ? 8 : 2;
     const int64_t fine = (records + least * hc::kAttendWaves - 1) / (least * hc::kAttendWaves);
     if (splits > fine) splits = fine;

@@ -737,11 +737,12 @@ struct Gathered {
 // Codes count from the middle, c - 8 in even slots and c - 7 in odd ones (numbers of the codes' own form; on the average the
 // middle itself), the rest is lo + 8 s or lo + 7 s: with codes from 0 the two sums would grow with the number of slots and nearly
 // cancel where a block's values lie around zero, each with roundings of its own.
-template <int NB, int NQ, int NP>
-__device__ __forceinline__ void values_by_codes(const uint8_t *at, const Queries<NB, NQ> &q, int lane, int slot0, int length, bool masked, const f32x4 &zero,
-                                                float (&p)[8], Gathered<NB> &s)
+// seen, held: a bit for each of the lane's slots, for the column and for the sequence; looked at where masked.
+template <int NB, int NP>
+__device__ __forceinline__ void values_by_codes(const uint8_t *at, int lane, bool masked, uint32_t seen, uint32_t held, float (&p)[8], Gathered<NB> &s)
 {
     constexpr bool kFineValues = NP == 3;
+    const f32x4 zero = kept_zero();
     const int n16 = lane & 15;
     ValuePart<NB> v;
     take_values<NB>(at, lane, v);
@@ -756,7 +757,7 @@ __device__ __forceinline__ void values_by_codes(const uint8_t *at, const Queries
         // slots that only some columns see, or none: a NaN there reaches those that see it by p s_b
         if (masked)
             for (int i = 0; i < 8; ++i)
-                if (slot0 + i >= length || !(mid[i] == mid[i])) mid[i] = 0.0f;
+                if (!(held >> i & 1) || !(mid[i] == mid[i])) mid[i] = 0.0f;
         split_bf16<NP>(mid, middle);
     }
     split_bf16<NP>(p, w);
@@ -767,8 +768,8 @@ __device__ __forceinline__ void values_by_codes(const uint8_t *at, const Queries
         float ps[8];
         for (int i = 0; i < 8; ++i) ps[i] = fmaf((float)v.steps[b][i], p[i], 0.0f);
         if (masked) {
-            const int from = kept_here(slot0);
-            for (int i = 0; i < 8; ++i) ps[i] = sees(q, from + i) ? ps[i] : 0.0f;
+            const uint32_t those = (uint32_t)kept_here((int)seen);
+            for (int i = 0; i < 8; ++i) ps[i] = (those >> i & 1) ? ps[i] : 0.0f;
         }
         split_bf16<NP>(ps, w);
         const u32x4 codes = v.codes[b >> 1];
@@ -785,6 +786,18 @@ __device__ __forceinline__ void values_by_codes(const uint8_t *at, const Queries
             for (int r = 0; r < 4; ++r) s.o[b >> 1][2 * (b & 1) + n][r] += fmaf(o[r], kFineValues || n ? 0x1p72f : 0x1p76f, base);
         }
     }
+}
+
+// The same as a call of its own, for the records of 16-bit caches that need it: in line it would cost the usual record's registers.
+template <int NB>
+struct Apart {
+    float p[8];
+    Gathered<NB> sums;
+};
+template <int NB>
+__device__ __attribute__((noinline)) void values_apart(const uint8_t *at, int lane, bool masked, uint32_t seen, uint32_t held, Apart<NB> *x)
+{
+    values_by_codes<NB, 2>(at, lane, masked, seen, held, x->p, x->sums);
 }
 
 // Values as float16 numbers, where all of a record's blocks are for float16 (for 16-bit results): p in one part, two for float16 results.
@@ -827,7 +840,7 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
     }
     // Values for float16?  The lanes look at the blocks together, and leave the lowest numbers as float16 behind the record.
     bool numbers = false;
-    if (TY != kF32 && !masked) {
+    if (TY != kF32) {
         bool fine = true;
         for (int i = 0; i < (NB + 3) / 4; ++i) {
             const int pair = 64 * i + lane;
@@ -844,15 +857,22 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
     float p[8], most = kNegInf;
     const float bias = 7.0f - s.top;      // (nothing seen yet: +infinity, which asks for a reference)
     for (int i = 0; i < 8; ++i) p[i] = fmaf(x[i >> 2][i & 3], q.factor, bias);
+    uint32_t seen = 0xff, held = 0xff;
     if (masked) {
         const int from = kept_here(slot0);
-        for (int i = 0; i < 8; ++i) p[i] = sees(q, from + i) ? p[i] : kNegInf;
+        seen = held = 0;
+        for (int i = 0; i < 8; ++i) {
+            const bool sees_it = sees(q, from + i);
+            p[i] = sees_it ? p[i] : kNegInf;
+            seen |= sees_it ? 1u << i : 0u;
+            held |= from + i < length ? 1u << i : 0u;
+        }
     }
     for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
     if (__builtin_amdgcn_ballot_w64(most > 15.0f) != 0) {
         most = kNegInf;
         for (int i = 0; i < 8; ++i)
-            if (!masked || sees(q, slot0 + i)) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
+            if (seen >> i & 1) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
         const float now = fmaxf(s.top, most);
@@ -862,14 +882,23 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
         for (int r = 0; r < 4; ++r)
             for (int i = 0; i < NB / 2; ++i)
                 for (int n = 0; n < 4; ++n) s.o[i][n][r] *= shrink;
-        for (int i = 0; i < 8; ++i) p[i] = !masked || sees(q, slot0 + i) ? fmaf(x[i >> 2][i & 3], q.factor, 7.0f - now) : kNegInf;
+        for (int i = 0; i < 8; ++i) p[i] = (seen >> i & 1) ? fmaf(x[i >> 2][i & 3], q.factor, 7.0f - now) : kNegInf;
     }
     for (int i = 0; i < 8; ++i) {
         p[i] = __builtin_amdgcn_exp2f(p[i]);
         s.total += p[i];
     }
-    if (TY != kF32 && numbers) values_by_numbers<NB, TY == kF16 ? 2 : 1>(at, at + record_bytes(NB), under, lane, p, s);
-    else values_by_codes<NB, NQ, TY == kF32 ? 3 : 2>(at, q, lane, slot0, length, masked, zero, p, s);
+    if constexpr (TY == kF32) {
+        values_by_codes<NB, 3>(at, lane, masked, seen, held, p, s);
+    } else if (numbers) {
+        values_by_numbers<NB, TY == kF16 ? 2 : 1>(at, at + record_bytes(NB), under, lane, p, s);
+    } else {
+        Apart<NB> x;
+        for (int i = 0; i < 8; ++i) x.p[i] = p[i];
+        x.sums = s;
+        values_apart<NB>(at, lane, masked, seen, held, &x);
+        s = x.sums;
+    }
 }
 
 template <int NB, int TY, bool FINE>
@@ -1331,10 +1360,13 @@ __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
     write_result<NB, TY>(a, h, first, tile * kColumns + column, place, top, total, x);
 }
 
-// The attention each slot received.  A wave holds kHeldRecords records' keys in LDS and goes over all columns of their sequence and head,
-// computing the scores again, and adds in the columns' order.  (Keeping the scores of the attention kernel instead would write and
-// read 4 bytes for every column and slot: with four columns 32 bytes a slot, with eight 64, against the 80 of the keys of 128 values.)
-constexpr int kHeldRecords = 4;
+// The attention each slot received.  A wave holds two records' keys in LDS (the next two on their way) and goes over all columns of their
+// sequence and head, computing the scores again, and adds in the columns' order.  (Keeping the scores of the attention kernel instead
+// would write and read 4 bytes for every column and slot: with four columns 32 bytes a slot, with eight 64, against the 80 of the keys of
+// 128 values.)  Between reading a cache's keys and computing: 25000 records and four columns take 28 us, 34 where a workgroup ends after
+// eight records (its start - positions, page, queries - costs as much as four), 40000 columns of 2048 rows on 5000 records 2 ms.
+// Four or eight records held: the same for few columns, 8 and 20 % slower for many (fewer waves fit).
+constexpr int kHeldRecords = 2, kWeightsPerUnit = 2;   // workgroups for a compute unit, where there are batches for more
 
 // The keys of a record: codes, steps, lowest numbers, in 16-byte pieces lane, lane + 64, ..
 template <int NB>
@@ -1377,64 +1409,88 @@ __device__ __forceinline__ float sum_over_row(const float *v, int n)
 }
 
 template <int NB, int TY>
-__global__ __launch_bounds__(256) void k_cache_weights(AttendArgs a, int records)
+__global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_weights(AttendArgs a, int records, int batches)
 {
-    constexpr int NQ = query_parts<TY>(), kBytes = 640 * NB;
+    constexpr int NQ = query_parts<TY>(), kBytes = 640 * NB, kBatch = kAttendWaves * kHeldRecords;
     __shared__ __align__(16) uint8_t s_mem[kAttendWaves][kHeldRecords][kBytes];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const uint32_t groups = ((uint32_t)records + kAttendWaves * kHeldRecords - 1) / (kAttendWaves * kHeldRecords);
-    const int it0 = (int)(blockIdx.x % groups) * (kAttendWaves * kHeldRecords) + wave * kHeldRecords;
-    const int h = (int)(blockIdx.x / groups % (unsigned)a.c.kv_heads);
-    const int s = (int)(blockIdx.x / groups / (unsigned)a.c.kv_heads);
+    const uint32_t groups = ((uint32_t)records + (uint32_t)(kBatch * batches) - 1) / (uint32_t)(kBatch * batches);
+    const int unit = (int)(blockIdx.x / groups), h = unit % a.c.kv_heads, s = unit / a.c.kv_heads;
+    const int begin = (int)(blockIdx.x % groups) * kBatch * batches + wave * kHeldRecords;
     const Rows rows = rows_of(a.starts, s, a.n_rows);
     const int first = rows.first, count = rows.count < a.max_rows ? rows.count : a.max_rows;
     const int length = sequence_length(a.c, s), slot0 = length - rows.behind;   // slot of the first row (in front of 0: more rows than slots)
-    if (it0 * kRecordSlots >= length) return;
-    bool there[kHeldRecords];
+    const int own = 8 * g + 4 * (n & 1) + (n & 2) + ((n >> 2) & 1);   // the lane's slot of a record's weights
+    const uint64_t line = ((uint64_t)s * a.c.kv_heads + h) * a.weight_stride;
     RawKeys<NB> raw[kHeldRecords];
-    for (int k = 0; k < kHeldRecords; ++k) {
-        const uint8_t *rec = (it0 + k) * kRecordSlots < length ? record_of(a.c, a.c.table, a.c.table_stride, s, h, (it0 + k) * kRecordSlots, NB) : nullptr;
-        there[k] = rec != nullptr;
-        if (rec) load_raw_keys<NB>(rec, lane, raw[k]);
-    }
-    for (int k = 0; k < kHeldRecords; ++k)
-        if (there[k]) lay_keys<NB>(s_mem[wave][k], lane, raw[k]);
-    wave_lds_order();
-    float sum[kHeldRecords][8];
-    for (int k = 0; k < kHeldRecords; ++k)
-        for (int i = 0; i < 8; ++i) sum[k][i] = 0.0f;
-    for (int tile = 0; tile * kColumns < count * a.group; ++tile) {
-        int from, to;
-        seen_records(a, count, slot0, length, tile, &from, &to);
-        if (it0 + kHeldRecords <= from || it0 >= to) continue;
-        const int column = tile * kColumns + n;
-        Queries<NB, NQ> q;
-        load_queries<NB, TY, kFine>(a, h, first, count, slot0, length, column, g, q);
-        float lse = 0.0f;
-        if (column < count * a.group) {
-            const int row = column / a.group, head = column - row * a.group;
-            lse = a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)];
+    float before[kHeldRecords];
+    uint32_t coming = 0;   // a bit for each record that is there
+    auto load_batch = [&](int it0) __attribute__((always_inline)) {
+        coming = 0;
+        for (int k = 0; k < kHeldRecords; ++k) {
+            const uint8_t *rec = (it0 + k) * kRecordSlots < length ? record_of(a.c, a.c.table, a.c.table_stride, s, h, (it0 + k) * kRecordSlots, NB) : nullptr;
+            if (!rec) continue;
+            coming |= 1u << k;
+            load_raw_keys<NB>(rec, lane, raw[k]);
         }
         for (int k = 0; k < kHeldRecords; ++k) {
-            if (!there[k]) continue;
-            KeyPart<NB> keys;
-            take_keys<NB, 512, 576>(s_mem[wave][k], lane, keys);
-            f32x4 x[2];
-            record_scores<NB, NQ, true>(keys, q, f32x4{0, 0, 0, 0}, x);
-            const int from_slot = (it0 + k) * kRecordSlots + 8 * g;
-            for (int i = 0; i < 8; ++i)
-                if (sees(q, from_slot + i))
-                    sum[k][i] += __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, lse * -kLog2e));
+            const int slot = (it0 + k) * kRecordSlots + own;
+            before[k] = a.prior && n < 8 && slot < length ? a.prior[line + (uint64_t)slot] : 0.0f;
         }
-    }
-    const int i = 4 * (n & 1) + (n & 2) + ((n >> 2) & 1);
-    for (int k = 0; k < kHeldRecords; ++k) {
-        const float all = sum_over_row(sum[k], n);
-        const int slot = (it0 + k) * kRecordSlots + 8 * g + i;
-        if (n < 8 && slot < length) {
-            const uint64_t at = ((uint64_t)s * a.c.kv_heads + h) * a.weight_stride + (uint64_t)slot;
-            a.weights[at] = (a.prior ? a.prior[at] : 0.0f) + all;
+    };
+    load_batch(begin);
+    int tile = -1;
+    Queries<NB, NQ> q;
+    float lse = 0.0f;
+    for (int it0 = begin; it0 < begin + kBatch * batches && it0 * kRecordSlots < length; it0 += kBatch) {
+        // the columns of the next tile that sees any of the records (a single tile stays)
+        int next = -1;
+        auto next_tile = [&]() __attribute__((always_inline)) {
+            int from = 0, to = 0;
+            do {
+                if (++next * kColumns >= count * a.group) return false;
+                seen_records(a, count, slot0, length, next, &from, &to);
+            } while (it0 + kHeldRecords <= from || it0 >= to);
+            if (next == tile) return true;
+            tile = next;
+            const int column = tile * kColumns + n;
+            load_queries<NB, TY, kFine>(a, h, first, count, slot0, length, column, g, q);
+            lse = 0.0f;
+            if (column < count * a.group) {
+                const int row = column / a.group, head = column - row * a.group;
+                lse = a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)];
+            }
+            return true;
+        };
+        bool more = next_tile();
+        const uint32_t there = coming;
+        float sum[kHeldRecords][8], prior[kHeldRecords];
+        for (int k = 0; k < kHeldRecords; ++k) {
+            if (there >> k & 1) lay_keys<NB>(s_mem[wave][k], lane, raw[k]);
+            prior[k] = before[k];
+            for (int i = 0; i < 8; ++i) sum[k][i] = 0.0f;
         }
+        wave_lds_order();
+        if (it0 + kBatch < begin + kBatch * batches) load_batch(it0 + kBatch);
+        for (; more; more = next_tile()) {
+            for (int k = 0; k < kHeldRecords; ++k) {
+                if (!(there >> k & 1)) continue;
+                KeyPart<NB> keys;
+                take_keys<NB, 512, 576>(s_mem[wave][k], lane, keys);
+                f32x4 x[2];
+                record_scores<NB, NQ, true>(keys, q, f32x4{0, 0, 0, 0}, x);
+                const int from_slot = (it0 + k) * kRecordSlots + 8 * g;
+                for (int i = 0; i < 8; ++i)
+                    if (sees(q, from_slot + i))
+                        sum[k][i] += __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, lse * -kLog2e));
+            }
+        }
+        for (int k = 0; k < kHeldRecords; ++k) {
+            const float all = sum_over_row(sum[k], n);
+            const int slot = (it0 + k) * kRecordSlots + own;
+            if (n < 8 && slot < length) a.weights[line + (uint64_t)slot] = prior[k] + all;
+        }
+        wave_lds_order();
     }
 }
 
@@ -1681,8 +1737,11 @@ static hipError_t attend_of(const AttendArgs &a, hipStream_t s)
     }
     if (e == hipSuccess && a.weights) {
         const uint32_t records = ((uint32_t)a.c.max_slots + kRecordSlots - 1) / kRecordSlots;
-        const uint32_t groups = (records + kAttendWaves * kHeldRecords - 1) / (kAttendWaves * kHeldRecords);
-        hipLaunchKernelGGL((k_cache_weights<NB, TY>), dim3(groups * (uint32_t)a.c.kv_heads * (uint32_t)a.c.n_seqs), dim3(256), 0, s, a, (int)records);
+        const uint32_t all = (records + kAttendWaves * kHeldRecords - 1) / (kAttendWaves * kHeldRecords);   // batches of a sequence and head
+        const uint32_t units = (uint32_t)a.c.kv_heads * (uint32_t)a.c.n_seqs;
+        uint32_t batches = all * units / (256 * kWeightsPerUnit);
+        if (batches < 1) batches = 1;
+        hipLaunchKernelGGL((k_cache_weights<NB, TY>), dim3((all + batches - 1) / batches * units), dim3(256), 0, s, a, (int)records, (int)batches);
         e = hipGetLastError();
     }
     return e;
