@@ -100,7 +100,7 @@ typedef struct homcomp_attention {
     float scale;              /* finite */
     int causal;
     size_t window;            /* 0: none */
-    float *d_lse;             /* [n_rows][q_heads], optional */
+    float *d_lse;             /* [n_rows][q_heads], optional; memory of its own */
     const float *d_prior;     /* [n_seqs][kv_heads][weight_stride], optional */
     float *d_weights;         /* the same, optional */
     size_t weight_stride;     /* at least max_length where weights are asked for */
@@ -130,7 +130,7 @@ typedef struct homcomp_eviction {
     size_t to_table_stride;
     int32_t *d_to_lengths;    /* [n_seqs]; not d_lengths */
     float *d_to_weights;      /* [n_seqs][kv_heads][keep]; not d_weights */
-    int32_t *d_kept;          /* [n_seqs][kv_heads][keep] */
+    int32_t *d_kept;          /* [n_seqs][kv_heads][keep]; neither of the two */
 } homcomp_eviction;
 
 int homcomp_cache_evict(const homcomp_cache *cache, const homcomp_eviction *eviction, void *stream);

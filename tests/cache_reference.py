@@ -80,13 +80,15 @@ def attention(q, keys, vals, there, lengths, starts, group, scale, causal, windo
     Bounds.  One score: a product of 32 terms in 32 bits, one multiply-add per block, the product of the lo part (its 24 terms), two
     multiplications for the scale: under 64 + nb roundings of at most 2^-24 of M = |scale| sum |q| (s c + |lo|).  So |dS| <= (64 + nb) 2^-24 M = e.
     A weight exp(S - lse) is off by a factor of at most 1 + 2 e + 2^-20 (both exponents' errors; the power's own error and the running sum's
-    L roundings are counted as 2^-20 + L 2^-24).  The output adds L terms w (s c + |lo|), each rounded to `parts` bfloat16 numbers:
-    2^-8, 2^-16 or 2^-24 of it; then one rounding to the output's type."""
+    L roundings are counted as 2^-20 + L 2^-24).  The output adds L terms w (s c + |lo|), then there is one rounding to the output's type.
+    For 16-bit results a term is a product of w and x' as float16 numbers, 2^-11 of it for either rounding (of w: one part for bfloat16
+    results, two for float16 ones, 2^-22), or of w in bfloat16 parts, 2^-8 or 2^-16: under 2^-8 and 2^-11 + 2^-16 in all; where numbers are
+    below float16's normal ones 2^-24, which is under 2^-13 of a block's largest (s is at least 2^-13 there) and inside what 2 max |v| leaves.  For 32-bit results 2^-24."""
     heads, d = q.shape[1], q.shape[2]
     out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
     d_out, d_lse = np.zeros(q.shape), np.zeros(q.shape[:2])
     weights, d_weights = [], []
-    part = {"bf16": 2.0 ** -8, "f16": 2.0 ** -16, "f32": 2.0 ** -24}[type_]
+    part = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11 + 2.0 ** -16, "f32": 2.0 ** -24}[type_]
     for s, L in enumerate(lengths):
         first, n = starts[s], starts[s + 1] - starts[s]
         w = np.zeros((heads // group, L)) if prior is None else prior[s, :, :L].astype(np.float64).copy()
@@ -112,7 +114,7 @@ def attention(q, keys, vals, there, lengths, starts, group, scale, causal, windo
                     e = (64 + d / 32) * 2.0 ** -24 * size.max()
                     run = 2.0 ** -20 + L * 2.0 ** -24
                     d_lse[first + i, g] = e + run + abs(z) * 2.0 ** -22
-                    big = p @ (np.abs(v) + 2 * np.abs(v).max(-1, keepdims=True))
+                    big = p @ (np.abs(v) + 2 * np.nanmax(np.abs(v), -1, keepdims=True))   # (a block of NaNs says nothing about the others)
                     d_out[first + i, g] = big * (part + 2 * (e + run)) + EPS[type_] * np.abs(out[first + i, g])
                     w[h, see] += p
                     dw[h, see] += p * (2 * e + run + abs(z) * 2.0 ** -22) + 2.0 ** -23 * w[h, see]

@@ -57,11 +57,13 @@ class Batch:
         self.d_lengths = world.put(np.array(self.lengths, np.int32))
         self.d_starts = world.put(self.starts)
 
-    def fill(self, scale=1.0):
-        """Stores random rows in all slots of all sequences."""
+    def fill(self, scale=1.0, edit=None):
+        """Stores random rows in all slots of all sequences; edit(k, v, slot of each row) may change them before."""
         total = sum(max(0, n) for n in self.lengths)
         k = (self.rng.standard_normal((total, self.heads, self.d)) * scale + self.rng.standard_normal((1, self.heads, self.d)) * 2).astype(np.float32)
         v = (self.rng.standard_normal((total, self.heads, self.d)) * scale).astype(np.float32)
+        if edit:
+            edit(k, v, np.concatenate([np.arange(max(0, n)) for n in self.lengths]))
         starts = self.w.put(np.concatenate([[0], np.cumsum([max(0, n) for n in self.lengths])]).astype(np.int32))
         self.c.store(self.w.put(k), self.w.put(v), self.d_table, self.d_lengths, starts)
 
@@ -129,9 +131,9 @@ def check_store(world, lengths, rows, heads, d, page, type_, seed=0, make=None, 
 
 
 def check_attend(world, lengths, rows, heads, group, d, page, type_, causal=True, window=0, scale=None, weights=False, in_place=False, seed=0,
-                 padding=0, bad_pages=(), strided=False, q_scale=1.0, tight=True, q_edit=None, fill_scale=1.0, prior=True):
+                 padding=0, bad_pages=(), strided=False, q_scale=1.0, tight=True, q_edit=None, fill_scale=1.0, prior=True, edit=None):
     b = Batch(world, lengths, rows, heads, d, page, seed, padding=padding, bad_pages=bad_pages)
-    b.fill(fill_scale)
+    b.fill(fill_scale, edit)
     q = torch.from_numpy((b.rng.standard_normal((b.total, heads * group, d)) * q_scale).astype(np.float32)).to(TYPES[type_])
     if q_edit:
         q_edit(q)
@@ -228,3 +230,89 @@ def check_evict(world, lengths, heads, d, page, keep, first=0, recent=0, seed=0,
     for p in range(b.n_pages):
         assert p in used or np.array_equal(now[p], old[p]), "a page that was not named changed"
     return b
+
+
+# Rows of keys and values that do not fit float16 numbers, or are none: what kernels take another way for.
+def huge_values(k, v, slots):
+    v[slots // 32 % 3 == 1] *= 9e3
+
+
+def tiny_values(k, v, slots):
+    v[slots // 32 % 2 == 0] *= 1e-6
+    v[slots % 32 == 7] = 1e-9      # a block of one small number: s = 0
+
+
+def tiny_keys(k, v, slots):
+    k[slots // 32 % 2 == 1] *= 1e-6
+
+
+def late_nan(k, v, slots):
+    """Only the last two rows of a causal batch see it."""
+    v[slots >= slots.max() - 1, 0, 3] = np.nan
+
+
+def late_nan_key(k, v, slots):
+    k[slots >= slots.max() - 1, 0, 3] = np.inf
+
+
+def check_run(world, heads=2, group=3, d=64, page=32, type_="bf16", seed=3, first=(37, 5, 50), steps=3, keep=24):
+    """As a server would: prompts stored and attended with their weights counted, tokens one by one, eviction to other pages, more tokens."""
+    rng = np.random.default_rng(seed)
+    n, t = len(first), TYPES[type_]
+    width = -(-(max(first) + 2 * steps) // page)
+    order = rng.permutation(2 * n * width + 1)
+    table = order[:n * width].reshape(n, width).astype(np.int32)
+    other = order[n * width:2 * n * width].reshape(n, width).astype(np.int32)
+    pages = world.full((len(order), world.cache.page_bytes(heads, d, page)), 255, torch.uint8)
+    c = world.cache.Cache(pages, heads, d, page)
+    most = width * page
+    d_table, d_other = world.put(table), world.put(other)
+    weights = world.full((n, heads, most), 0.0, torch.float32)
+    book = np.zeros((n, heads, most))
+    slack = np.zeros((n, heads, most))
+    lengths = np.zeros(n, np.int32)
+
+    def step(rows):
+        nonlocal lengths
+        lengths = (lengths + rows).astype(np.int32)
+        starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        k, v = (torch.from_numpy(rng.standard_normal((starts[-1], heads, d)).astype(np.float32)).to(t) for _ in range(2))
+        q = torch.from_numpy(rng.standard_normal((starts[-1], heads * group, d)).astype(np.float32)).to(t)
+        d_lengths, d_starts = world.put(lengths), world.put(starts)
+        c.store(world.put(k), world.put(v), d_table, d_lengths, d_starts)
+        out = world.full(tuple(q.shape), 0.0, t)
+        need = c.scratch_bytes(len(q), heads * group, n, width, t, weights=True)
+        c.attend(world.put(q), out, d_table, d_lengths, d_starts, weights=weights, prior=weights, scratch=world.full((need // 4 + 4,), float("nan"), torch.float32))
+        raw = ref.Pages(world.get(pages), heads, d, page)
+        held = [[raw.rows(now[s], h, int(L)) for h in range(heads)] for s, L in enumerate(lengths)]
+        part = [[[x[i] for x in per] for per in held] for i in range(3)]
+        want, _, w, tol, _, tol_w = ref.attention(q.double().numpy(), *part, lengths, starts, group, d ** -0.5, True, 0, type_, book)
+        close(world.get(out), want, tol, "out")
+        got = world.get(weights)
+        for s, L in enumerate(lengths):
+            slack[s, :, :L] += tol_w[s]
+            close(got[s, :, :L], w[s], slack[s, :, :L], "weights")
+            book[s, :, :L] = w[s]
+
+    now = table
+    step(np.array(first))
+    for _ in range(steps):
+        step(np.ones(n, np.int32))
+    to_lengths = world.full((n,), 0, torch.int32)
+    old = world.get(weights)
+    to_weights, kept = c.evict(weights, d_table, world.put(lengths), keep, d_other, to_lengths, first=2, recent=8,
+                               to_weights=world.full((n, heads, keep), 0.0, torch.float32), kept=world.full((n, heads, keep), 0, torch.int32))
+    stays = ref.evict(old, lengths, keep, 2, 8)
+    got, got_w = world.get(kept), world.get(to_weights)
+    book[:], slack[:] = 0.0, 0.0
+    for s, L in enumerate(lengths):
+        for h in range(heads):
+            row = stays[s * heads + h]
+            assert got[s, h, :len(row)].tolist() == row
+            book[s, h, :len(row)] = old[s, h][row]
+    lengths = world.get(to_lengths).astype(np.int32)
+    assert lengths.tolist() == [min(keep, n + steps) for n in first]
+    now, d_table = other, d_other
+    weights = world.put(book, torch.float32)
+    for _ in range(steps):
+        step(np.resize([1, 0, 2], n))

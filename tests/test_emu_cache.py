@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from cache_world import World, check_attend, check_evict, check_store
+from cache_world import (World, check_attend, check_evict, check_run, check_store, huge_values, late_nan, late_nan_key, tiny_keys,
+                         tiny_values)
 
 
 @pytest.fixture(scope="module")
@@ -76,6 +77,35 @@ def test_store_hard_blocks(world, type_):
 ])
 def test_attend(world, lengths, rows, heads, group, d, page, type_, kw):
     check_attend(world, lengths, rows, heads, group, d, page, type_, **kw)
+
+
+# Many columns: records unpacked once for several tiles of sixteen, and what falls back from there.
+@pytest.mark.parametrize("lengths,rows,heads,group,d,page,type_,kw", [
+    ([100], [33], 1, 2, 64, 32, "bf16", {}),                                    # 5 tiles
+    ([70, 33], [40, 2], 1, 4, 64, 32, "f16", dict(padding=1)),                  # 10 tiles, of the second sequence one
+    ([40], [20], 1, 2, 256, 32, "bf16", dict(strided=True)),
+    ([300], [9], 1, 2, 64, 32, "f16", dict(window=30)),                         # parts
+    ([90], [9], 1, 4, 64, 32, "bf16", dict(causal=False, weights=True)),
+    ([130], [10], 1, 3, 64, 32, "bf16", dict(edit=huge_values)),
+    ([130], [10], 1, 3, 64, 32, "f16", dict(edit=tiny_values, weights=True)),
+    ([130], [10], 1, 3, 64, 32, "bf16", dict(edit=tiny_keys)),
+    ([70], [8], 1, 3, 64, 32, "bf16", dict(edit=late_nan)),
+    ([70], [8], 1, 3, 64, 32, "f16", dict(edit=late_nan_key, weights=True)),
+    ([100], [10], 1, 3, 64, 32, "bf16", dict(bad_pages=[(0, 1, 99)])),
+])
+def test_attend_many_columns(world, lengths, rows, heads, group, d, page, type_, kw):
+    check_attend(world, lengths, rows, heads, group, d, page, type_, **kw)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("edit", [huge_values, tiny_values, tiny_keys, late_nan, late_nan_key])
+def test_attend_hard_rows(world, edit, type_):
+    check_attend(world, [100], [3], 1, 2, 64, 32, type_, edit=edit)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f32"])
+def test_operators_together(world, type_):
+    check_run(world, type_=type_)
 
 
 @pytest.mark.parametrize("lengths,heads,d,page,keep,first,recent", [

@@ -66,8 +66,12 @@ def new_pages(n_pages: int, kv_heads: int, head_dim: int, page_tokens: int, devi
 
 def _stream_of(device, stream) -> int:
     import torch
+    if device.type != "cuda":
+        raise ValueError("the cache's pages lie in a GPU's memory")
     if stream is None:   # the handle alone, without the object around it: a tenth of the time
         return torch._C._cuda_getCurrentRawStream(device.index)
+    if stream.device != device:
+        raise ValueError("stream: of the pages' device")
     return int(stream.cuda_stream)
 
 

@@ -189,6 +189,7 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t,
     if (!aligned(t->d_lse, 4) || !aligned(t->d_prior, 4) || !aligned(t->d_weights, 4) || !aligned(t->d_scratch, 16)) return HOMCOMP_ERR_ALIGNMENT;
     if (p.tiles > 0) {
         if (!t->d_q || !t->d_out || t->d_q == t->d_out) return HOMCOMP_ERR_INVALID_ARG;
+        if (t->d_lse && (t->d_lse == t->d_weights || t->d_lse == t->d_out)) return HOMCOMP_ERR_INVALID_ARG;
         if (!aligned(t->d_q, bytes_of(t->type)) || !aligned(t->d_out, bytes_of(t->type))) return HOMCOMP_ERR_ALIGNMENT;
     }
     const size_t need = p.partial_bytes + p.sums_bytes + p.lse_bytes + p.left_bytes;
@@ -238,7 +239,9 @@ int homcomp_cache_evict(const homcomp_cache *cache, const homcomp_eviction *t, v
         return HOMCOMP_ERR_INVALID_ARG;
     if (a.c.n_seqs == 0) return HOMCOMP_OK;
     if (!t->d_weights || !t->d_to_table || !t->d_to_lengths || !t->d_to_weights || !t->d_kept) return HOMCOMP_ERR_INVALID_ARG;
-    if (t->d_to_lengths == cache->d_lengths || t->d_to_weights == t->d_weights || t->d_to_table == cache->d_table) return HOMCOMP_ERR_INVALID_ARG;
+    if (t->d_to_lengths == cache->d_lengths || t->d_to_weights == t->d_weights || t->d_to_table == cache->d_table ||
+        (const void *)t->d_kept == t->d_weights || (const void *)t->d_kept == t->d_to_weights)
+        return HOMCOMP_ERR_INVALID_ARG;
     if (!aligned(t->d_weights, 4) || !aligned(t->d_to_table, 4) || !aligned(t->d_to_lengths, 4) || !aligned(t->d_to_weights, 4) || !aligned(t->d_kept, 4))
         return HOMCOMP_ERR_ALIGNMENT;
     a.weights = t->d_weights;
