@@ -92,6 +92,8 @@ def test_attend(world, lengths, rows, heads, group, d, page, type_, kw):
     ([70], [8], 1, 3, 64, 32, "bf16", dict(edit=late_nan)),
     ([70], [8], 1, 3, 64, 32, "f16", dict(edit=late_nan_key, weights=True)),
     ([100], [10], 1, 3, 64, 32, "bf16", dict(bad_pages=[(0, 1, 99)])),
+    ([320], [300], 1, 1, 64, 32, "bf16", dict(window=40)),                      # a tile sees a part of what its parts are cut from
+    ([320], [300], 1, 1, 64, 32, "bf16", dict(window=40, edit=huge_values)),
 ])
 def test_attend_many_columns(world, lengths, rows, heads, group, d, page, type_, kw):
     check_attend(world, lengths, rows, heads, group, d, page, type_, **kw)

@@ -109,6 +109,9 @@ def test_evict_ties_and_odd_weights(world):
     ([70], [8], 1, 3, 128, 32, dict(edit=late_nan_key, weights=True)),
     ([200], [10], 1, 3, 64, 32, dict(bad_pages=[(0, 1, 99), (0, 4, -1)])),
     ([20], [33], 1, 2, 64, 32, {}),                                     # more rows than slots
+    ([320], [300], 1, 1, 64, 32, dict(window=40)),                      # a tile sees a part of what its parts are cut from
+    ([320], [300], 1, 1, 128, 32, dict(window=40, edit=huge_values)),
+    ([600, 340], [300, 2], 2, 2, 64, 64, dict(window=260, weights=True, edit=tiny_values)),
 ])
 def test_attend_many_columns(world, lengths, rows, heads, group, d, page, type_, kw):
     check_attend(world, lengths, rows, heads, group, d, page, type_, **kw)

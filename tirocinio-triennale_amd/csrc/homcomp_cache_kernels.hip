@@ -655,11 +655,10 @@ __device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Querie
 }
 
 // Records that a tile's columns can see at all: [*from, *to).
-template <int COLUMNS = kColumns>
-__device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int slot0, int length, int tile, int *from, int *to)
+__device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int slot0, int length, int tile, int *from, int *to, int columns = kColumns)
 {
-    const int first_row = tile * COLUMNS / a.group;
-    int last_row = (tile * COLUMNS + COLUMNS - 1) / a.group;
+    const int first_row = tile * columns / a.group;
+    int last_row = (tile * columns + columns - 1) / a.group;
     if (last_row >= count) last_row = count - 1;
     int end = length, begin = 0;
     if (a.causal && slot0 + last_row + 1 < end) end = slot0 + last_row + 1;
@@ -667,6 +666,15 @@ __device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int
     if (end < 0) end = 0;
     *from = begin >> 5;
     *to = begin < end ? (end + 31) >> 5 : begin >> 5;
+}
+// The record a tile's parts are counted from: the first that it can see, or that the wide tile can which it belongs to (whose parts they
+// are then).
+__device__ __forceinline__ int parts_origin(const AttendArgs &a, int count, int slot0, int length, int tile)
+{
+    int from, to;
+    if (a.wide_tiles) seen_records(a, count, slot0, length, tile / a.tiles_in_wide, &from, &to, kColumns * a.tiles_in_wide);
+    else seen_records(a, count, slot0, length, tile, &from, &to);
+    return from;
 }
 // Slots that every one of a tile's columns sees: [*from, *to).
 template <int COLUMNS = kColumns>
@@ -926,9 +934,10 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     int from, to, all_from, all_to;
     seen_records(a, count, slot0, length, tile, &from, &to);
     seen_by_all(a, count, slot0, length, tile, &all_from, &all_to);
-    from += split * a.split_records;
-    if (split > 0 && from >= to) return;
-    if (to > from + a.split_records) to = from + a.split_records;
+    const int part_from = parts_origin(a, count, slot0, length, tile) + split * a.split_records;
+    if (split > 0 && part_from >= to) return;   // (one in front of what the tile sees is written all the same, with nothing in it)
+    if (from < part_from) from = part_from;
+    if (to > part_from + a.split_records) to = part_from + a.split_records;
 
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     Queries<NB, NQ> q;
@@ -1181,7 +1190,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
     const int length = sequence_length(a.c, s), slot0 = length - rows.behind;   // slot of the first row (in front of 0: more rows than slots)
     if (wide * kWide >= count * a.group) return;
     int from, to;
-    seen_records<kWide>(a, count, slot0, length, wide, &from, &to);
+    seen_records(a, count, slot0, length, wide, &from, &to, kWide);
     from += split * a.split_records;
     if (to > from + a.split_records) to = from + a.split_records;
 
@@ -1189,7 +1198,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
     WideGathered<NB> acc[CT];
     const int wave_tile = wide * W + wave;   // of 16 CT columns
     int own_from, own_to, all_from, all_to;
-    seen_records<kColumns * CT>(a, count, slot0, length, wave_tile, &own_from, &own_to);
+    seen_records(a, count, slot0, length, wave_tile, &own_from, &own_to, kColumns * CT);
     seen_by_all<kColumns * CT>(a, count, slot0, length, wave_tile, &all_from, &all_to);
     if (wave_tile * kColumns * CT >= count * a.group) own_to = own_from;
     for (int t = 0; t < CT; ++t) {
@@ -1329,7 +1338,7 @@ __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
     if (tile * kColumns + column >= count * a.group) return;
     int from, to;
     seen_records(a, count, slot0, length, tile, &from, &to);
-    int parts = (to - from + a.split_records - 1) / a.split_records;
+    int parts = (to - parts_origin(a, count, slot0, length, tile) + a.split_records - 1) / a.split_records;
     if (parts < 1) parts = 1;
     if (parts > a.splits) parts = a.splits;
     const uint64_t at = ((uint64_t)unit * kColumns + (uint32_t)column) * (uint32_t)a.splits;
