@@ -171,26 +171,33 @@ struct Block8 {
     uint32_t code[8];   // of a lane's eight values
     uint32_t s, lo;     // f16 and bf16 bits, the same in the block's four lanes
 };
-// Four adjacent lanes hold a block, eight values each.  All decisions are those of exact arithmetic: the borders lo + (j + 1/2) s
-// have at most 44 significant bits (s is at least a fifteenth of the range, lo at most 2^8 of its own last places), so 64-bit
-// floats hold them.  In 32 bits (x - lo) / s + 1/2 is at most 15 1/2 and off by four roundings (the difference, the reciprocal, the product,
-// the sum): under 64 * 2^-24 = 2^-18.  Only where a value is within 2^-17 of a border, in about one wave of a hundred, are the borders looked at.
+// Four adjacent lanes hold a block; what another of them has.
+template <int XOR>
+__device__ __forceinline__ uint32_t of_quad(uint32_t x)
+{
+    static_assert(XOR == 1 || XOR == 2, "a lane of the four");
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, XOR == 1 ? 0xb1 : 0x4e, 0xf, 0xf, true);
+}
+template <int XOR>
+__device__ __forceinline__ float of_quad(float x) { return __builtin_bit_cast(float, of_quad<XOR>(__builtin_bit_cast(uint32_t, x))); }
+
+// Eight values a lane.  All decisions are those of exact arithmetic: the borders lo + (j + 1/2) s have at most 44 significant bits (s is at
+// least a fifteenth of the range, lo at most 2^8 of its own last places), so 64-bit floats hold them.  In 32 bits (x - lo) / s + 1/2 is
+// at most 15 1/2 and off by the roundings of the difference and the sum and the reciprocal's 2^-23: under 64 * 2^-24 = 2^-18.
+// Only where a value is within 2^-17 of a border, in about one wave of a hundred, are the borders looked at.
 __device__ __forceinline__ Block8 quantise(const float *x)
 {
-    float mn = x[0], mx = x[0];
-    bool bad = false;
+    float mn = x[0], mx = x[0], odd = 0.0f;
     for (int i = 0; i < 8; ++i) {
         mn = fminf(mn, x[i]);
         mx = fmaxf(mx, x[i]);
-        bad = bad || !(fabsf(x[i]) <= 3.4028234663852886e38f);
+        odd = fmaf(x[i], 0.0f, odd);   // a NaN, where there is one or an infinity
     }
-    for (int d = 1; d < 4; d <<= 1) {
-        mn = fminf(mn, __shfl_xor(mn, d, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-    }
-    int any = bad ? 1 : 0;
-    any |= __shfl_xor(any, 1, 64);
-    any |= __shfl_xor(any, 2, 64);
+    if (!(odd == odd)) mx = __builtin_inff();   // (the block is none then)
+    mn = fminf(mn, of_quad<1>(mn));
+    mx = fmaxf(mx, of_quad<1>(mx));
+    mn = fminf(mn, of_quad<2>(mn));
+    mx = fmaxf(mx, of_quad<2>(mx));
     Block8 r;
     // toward minus infinity: cutting the low bits moves toward zero, a negative number that loses some goes one further
     const uint32_t bits = __builtin_bit_cast(uint32_t, mn);
@@ -200,28 +207,27 @@ __device__ __forceinline__ Block8 quantise(const float *x)
     r.s = f32_to_f16((float)range * (1.0f / 15.0f));   // (within one place of the quotient: put right below, upward and down)
     if ((r.s & 0x7fffu) < 0x7c00u && r.s > 0 && 15.0 * (double)f16_to_f32(r.s - 1) >= range) --r.s;
     if ((r.s & 0x7fffu) < 0x7c00u && 15.0 * (double)f16_to_f32(r.s) < range) ++r.s;
-    const bool none = any || !(range <= 1.0e38) || (r.s & 0x7fffu) >= 0x7c00u;
+    const bool none = !(range <= 1.0e38) || (r.s & 0x7fffu) >= 0x7c00u;
     if (none) {
         r.s = 0x7e00u;
         r.lo = 0;
     }
-    const float s = f16_to_f32(r.s), rs = s > 0.0f ? 1.0f / s : 0.0f;
+    const float s = f16_to_f32(r.s), rs = s > 0.0f ? __builtin_amdgcn_rcpf(s) : 0.0f;   // (0: all codes are)
     constexpr float near = 0x1p-17f;
-    float c[8];
-    bool close = false;
+    float far = 0.0f;   // from the middle between two borders
     for (int i = 0; i < 8; ++i) {
-        const float t = (x[i] - lo) * rs + 0.5f, f = floorf(t);
-        c[i] = fminf(fmaxf(f, 0.0f), 15.0f);
-        close = close || !(t - f > near && t - f < 1.0f - near);
+        const float t = fmaxf(fmaf(x[i] - lo, rs, 0.5f), 0.5f);   // (a NaN: 1/2)
+        r.code[i] = (uint32_t)t;
+        far = fmaxf(far, fabsf(__builtin_amdgcn_fractf(t) - 0.5f));
     }
-    if (close && s > 0.0f && !none) {
+    if (far > 0.5f - near) {
         for (int i = 0; i < 8; ++i) {
-            const double v = (double)x[i], at = (double)c[i];
-            if (at < 15.0 && v >= fma(at + 0.5, (double)s, (double)lo)) c[i] += 1.0f;
-            else if (at > 0.0 && v < fma(at - 0.5, (double)s, (double)lo)) c[i] -= 1.0f;
+            const uint32_t c = r.code[i];
+            const double v = (double)x[i], at = (double)c;
+            if (c < 15 && v >= fma(at + 0.5, (double)s, (double)lo)) r.code[i] = c + 1;
+            else if (c > 0 && v < fma(at - 0.5, (double)s, (double)lo)) r.code[i] = c - 1;
         }
     }
-    for (int i = 0; i < 8; ++i) r.code[i] = s > 0.0f && !none ? (uint32_t)(int)c[i] : 0u;
     return r;
 }
 
@@ -331,7 +337,7 @@ __global__ __launch_bounds__(256) void k_cache_store(CacheArgs c, RowsArgs a, ui
             // value m and value 16 + m of the block share a byte: lanes j and j ^ 2 exchange
             for (int n = 0; n < 4; ++n) {
                 const uint32_t give = j < 2 ? q.code[4 + n] : q.code[n];
-                const uint32_t got = (uint32_t)__shfl_xor((int)give, 2, 64);
+                const uint32_t got = of_quad<2>(give);
                 word[n] |= (j < 2 ? q.code[n] | (got << 4) : got | (q.code[4 + n] << 4)) << (8 * e);
             }
             if (j == ((2 * i + e) & 3)) step[(2 * i + e) >> 2] = q.s, low[(2 * i + e) >> 2] = q.lo;
