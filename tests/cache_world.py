@@ -116,8 +116,12 @@ def check_store(world, lengths, rows, heads, d, page, type_, seed=0, make=None, 
                     assert not (off > 1e-12 * np.abs(x)).any(), "the error bound s / 2"
     assert np.array_equal(after[~touched.reshape(-1)], before[~touched.reshape(-1)]), "bytes of other slots changed"
     # back as numbers, into arrays whose other rows stay as they are
-    outs = [world.full((b.total, heads, d), 77.0, TYPES[type_]) for _ in range(2)]
+    wide = [world.full((b.total, heads + 1, d + 3), 77.0, TYPES[type_]) for _ in range(2)]
+    outs = [x[:, :heads, 1:d + 1] for x in wide] if strided else [world.full((b.total, heads, d), 77.0, TYPES[type_]) for _ in range(2)]
     b.c.load(*outs, b.d_table, b.d_lengths, b.d_starts)
+    for x in wide if strided else []:
+        x = world.get(x)
+        assert (x[:, heads:] == 77.0).all() and (x[:, :, 0] == 77.0).all() and (x[:, :, d + 1:] == 77.0).all(), "what lies between rows was written"
     for out, want in zip(outs, expect):
         got = world.get(out)
         assert (got[~known] == 77.0).all(), "padding was written"
