@@ -1538,10 +1538,13 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t *sums, 
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t x = mine;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = (uint32_t)__shfl((int)x, lane >= d ? lane - d : lane, 64);
-        if (lane >= d) x += y;
-    }
+    // inside rows of sixteen lanes, then the rows' last lanes on into the rows behind
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
     if (lane == 63) sums[wave] = x;
     __syncthreads();
     uint32_t before = 0, total = 0;
@@ -1569,10 +1572,13 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
     const float *w = a.weights + unit * a.weight_stride;
     const int count = length < a.keep ? length : a.keep;
     const bool all = length <= a.keep;
-    const int low = a.first, high = length - a.recent;           // candidates: low <= slot < high
-    uint32_t need = (uint32_t)(a.keep - a.first - a.recent);     // of them to stay
+    uint32_t need = (uint32_t)(a.keep - a.first - a.recent);     // of the candidates, low <= slot < high, to stay
     const bool some = !all && need > 0, once = length <= kSelectTile;
+    const int low = all ? length : a.first, high = all ? length : length - a.recent;
+    // a key that is above all weights' for slots that stay anyway, and (not looked at) behind the last
+    constexpr uint32_t kStays = 0xffffffffu;
     float own[kSelectEach];
+    uint32_t key[kSelectEach];
     auto load = [&](int base) __attribute__((always_inline)) {
         const int j = base + tid * kSelectEach;
         if (j + kSelectEach <= length && ((uintptr_t)(w + j) & 15u) == 0) {
@@ -1580,9 +1586,12 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
         } else {
             for (int i = 0; i < kSelectEach; ++i) own[i] = j + i < length ? w[j + i] : 0.0f;
         }
+        for (int i = 0; i < kSelectEach; ++i) key[i] = j + i >= low && j + i < high ? weight_key(own[i]) : kStays;
     };
+    // (waves that hold nothing go from barrier to barrier)
+    const int wave_first = __builtin_amdgcn_readfirstlane(tid & ~63) * kSelectEach;
     load(0);
-    uint32_t prefix = 0, mask = 0;
+    uint32_t prefix = some ? 0 : kStays - 1, mask = 0;
     if (some) {
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
@@ -1592,11 +1601,9 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
             __syncthreads();
             for (int base = 0; base < length; base += kSelectTile) {
                 if (!once) load(base);
-                for (int i = 0; i < kSelectEach; ++i) {
-                    const int j = base + tid * kSelectEach + i;
-                    const uint32_t k = weight_key(own[i]);
-                    if (j >= low && j < high && (k & mask) == prefix) atomicAdd(&s_bins[(k >> shift) & digits], 1u);
-                }
+                if (base + wave_first >= length) continue;
+                for (int i = 0; i < kSelectEach; ++i)
+                    if (key[i] != kStays && (key[i] & mask) == prefix) atomicAdd(&s_bins[(key[i] >> shift) & digits], 1u);
             }
             __syncthreads();
             const uint32_t bin = (uint32_t)(kSelectBins - 1 - 2 * tid), c0 = s_bins[bin], c1 = s_bins[bin - 1];
@@ -1611,34 +1618,32 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
             prefix |= s_found[0] << shift;
             mask |= digits << shift;
             need = s_found[1];
-            __syncthreads();
         }
     }
     // all with a larger key than `prefix` stay, and `need` of those with that key, the ones in front
-    uint32_t kept = 0, equal = 0;
+    uint32_t greater = 0, equal = 0;   // in front of a tile
     for (int base = 0; base < length; base += kSelectTile) {
         if (!once) load(base);
-        const int j0 = base + tid * kSelectEach;
-        uint32_t same = 0, total;
-        for (int i = 0; i < kSelectEach; ++i)
-            if (some && j0 + i >= low && j0 + i < high && weight_key(own[i]) == prefix) same |= 1u << i;
-        uint32_t rank = equal + block_prefix((uint32_t)__builtin_popcount(same), s_sums, &total), stays = 0;
-        equal += total;
+        const int j0 = base + tid * kSelectEach, held = length - j0;
+        uint32_t more = 0, same = 0, total;
         for (int i = 0; i < kSelectEach; ++i) {
-            const int j = j0 + i;
-            bool stay = j < length && (all || j < low || j >= high);
-            if (some && j >= low && j < high) stay = weight_key(own[i]) > prefix || (((same >> i) & 1u) && rank < need);
-            rank += (same >> i) & 1u;
-            if (stay) stays |= 1u << i;
+            more |= key[i] > prefix ? 1u << i : 0u;
+            same |= key[i] == prefix ? 1u << i : 0u;
         }
-        uint32_t at = kept + block_prefix((uint32_t)__builtin_popcount(stays), s_sums, &total);
-        kept += total;
+        if (held < kSelectEach) more &= held > 0 ? (1u << held) - 1u : 0u;
+        const uint32_t front = block_prefix(((uint32_t)__builtin_popcount(more) << 16) | (uint32_t)__builtin_popcount(same), s_sums, &total);
+        uint32_t rank = equal + (front & 0xffffu), at = greater + (front >> 16) + (rank < need ? rank : need);
+        greater += total >> 16;
+        equal += total & 0xffffu;
+        if (base + wave_first >= length) continue;
         for (int i = 0; i < kSelectEach; ++i) {
-            if (((stays >> i) & 1u) && at < (uint32_t)count) {
+            const bool tied = (same >> i) & 1u;
+            if ((((more >> i) & 1u) || (tied && rank < need)) && at < (uint32_t)count) {
                 a.kept[unit * a.keep + at] = j0 + i;
                 a.to_weights[unit * a.keep + at] = own[i];
                 ++at;
             }
+            rank += tied ? 1u : 0u;
         }
     }
     for (int i = count + tid; i < a.keep; i += kSelectThreads) {
