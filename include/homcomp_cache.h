@@ -40,6 +40,8 @@
  *     to and are evicted as zeros.  A length is cut to what a row of the table can hold, a negative one is 0.  What lies behind a
  *     sequence's last slot is never part of a result.
  *   - Two calls that touch the same slots or the same scratch memory have to be ordered by the caller (one stream, or events).
+ *     Sequences may have pages in common; rows that one call writes must have slots of their own.
+ *   - A call of more workgroups than a launch can have (2^24 - 1 of 256 threads) is refused.
  */
 #ifndef HOMCOMP_CACHE_H
 #define HOMCOMP_CACHE_H
@@ -116,8 +118,8 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *at
 /* Eviction by the weights that homcomp_cache_attend gathers.  Of a sequence that holds L > keep slots every head keeps `keep` of its own
  * choice: the first `first`, the last `recent`, and of those between the keep - first - recent of the largest weight (of equal
  * ones those in front; a NaN counts as the smallest).  They go, in their order and as the bits they are, to the first slots of the pages
- * that d_to_table names.  A sequence of at most `keep` slots is moved whole.  The pages moved to must not be pages of any sequence's slots;
- * the old pages are left as they were.  n = min(L, keep):
+ * that d_to_table names.  A sequence of at most `keep` slots is moved whole.  The pages moved to must not be pages of any sequence's slots,
+ * nor named twice; the old pages are left as they were.  n = min(L, keep):
  *   to_lengths[s] = n     kept[s][h][i] = the old slot of row i < n, -1 for i >= n       to_weights[s][h][i] = its weight, 0 for i >= n
  */
 typedef struct homcomp_eviction {

@@ -106,6 +106,19 @@ def test_bad_caches_refused(cache, kw, want):
     assert L.homcomp_cache_evict(c, eviction(cache), 0) == want
 
 
+def test_calls_beyond_a_launch_are_refused(cache):
+    L, much = cache.lib(), dict(n_seqs=65535, kv_heads=1024)
+    c, scratch = the_cache(cache, **much), dict(scratch=AT, scratch_bytes=1 << 60)
+    assert L.homcomp_cache_attend(c, attention(cache, q_heads=1024, **scratch), 0) == INVALID
+    assert L.homcomp_cache_evict(c, eviction(cache), 0) == INVALID
+    assert rows_call(cache, "homcomp_cache_store", c) == INVALID
+    few = the_cache(cache, n_seqs=1, kv_heads=64)
+    assert rows_call(cache, "homcomp_cache_load", few, n_rows=(1 << 31) - 1) == INVALID
+    assert L.homcomp_cache_attend(few, attention(cache, q_heads=64, n_rows=1 << 24, max_rows=1 << 24, **scratch), 0) == INVALID
+    assert L.homcomp_cache_evict(the_cache(cache, n_seqs=16000, kv_heads=64),
+                                 eviction(cache, keep=1 << 20, to_table_stride=1 << 15), 0) == INVALID
+
+
 def test_null_structures_refused(cache):
     L = cache.lib()
     assert rows_call(cache, "homcomp_cache_store", None) == INVALID

@@ -351,3 +351,54 @@ def test_eviction_outside_graphs_leaves_inputs(world):
     assert to_lengths.tolist() == [20, 5, 20]
     same = (old == b.pages).all(1)
     assert same.tolist() == [p not in b.free[:2] for p in range(b.n_pages)]
+
+
+def test_nothing_held(world):
+    """No slots at all, by the table or by max_length: rows see nothing, no weight is written, nothing stays."""
+    b, (k, v, q), out, w = decode_setup(world, [90, 5, 64])
+    none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
+    for table, kw in ((none, {}), (b.d_table, dict(max_length=0))):
+        out.fill_(7.0)
+        lse, w = world.full((3, 8), 7.0, torch.float32), world.full((3, 2, 1), 33.0, torch.float32)
+        b.c.attend(q, out, table, b.d_lengths, b.d_starts, lse=lse, weights=w, **kw)
+        assert (out == 0).all() and torch.isneginf(lse).all() and (w == 33).all()
+        to_lengths = world.full((3,), 9, torch.int32)
+        to_w, kept = b.c.evict(w, table, b.d_lengths, 20, torch.tensor([[b.free[0]]] * 3, dtype=torch.int32, device="cuda"), to_lengths, **kw)
+        assert to_lengths.tolist() == [0, 0, 0] and (kept == -1).all() and (to_w == 0).all()
+    old = b.pages.clone()
+    b.c.store(k, v, none, b.d_lengths, b.d_starts)
+    k.fill_(7.0)
+    b.c.load(k, v, none, b.d_lengths, b.d_starts)
+    assert torch.equal(old, b.pages) and (k == 7).all()
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("group", [2, 20])
+def test_queries_that_are_none(world, type_, group):
+    """A row of NaNs gives NaNs and nothing else changes; a row of zeros the mean."""
+    def edit(q):
+        q[0, 0] = float("nan")
+        q[1, :, ::2] = 0.0
+        q[2] = 0.0
+    check_attend(world, [90, 40], [2, 2], 1, group, 64, 32, type_, q_edit=edit)
+
+
+def test_memory_for_a_stream_comes_from_it(world):
+    """Scratch memory and results that a call makes for another stream are that stream's."""
+    seen = []
+
+    class Watched(torch.Tensor):
+        def new_empty(self, *a, **kw):
+            seen.append(torch.cuda.current_stream())
+            return self.as_subclass(torch.Tensor).new_empty(*a, **kw)
+
+    b, (k, v, q), out, w = decode_setup(world, [1500, 700], room=1504)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    b.c.attend(q.as_subclass(Watched), out, b.d_table, b.d_lengths, b.d_starts, weights=w, stream=s)
+    to = torch.tensor([[b.free[0]], [b.free[1]]], dtype=torch.int32, device="cuda")
+    to_lengths = world.full((2,), 0, torch.int32)
+    torch.cuda.synchronize()
+    b.c.evict(w.as_subclass(Watched), b.d_table, b.d_lengths, 20, to, to_lengths, stream=s)
+    torch.cuda.synchronize()
+    assert seen == [s, s, s]

@@ -11,6 +11,7 @@ refusal is a ValueError or a TypeError, and nothing has been enqueued then.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import struct
 
@@ -73,6 +74,17 @@ def _stream_of(device, stream) -> int:
     if stream.device != device:
         raise ValueError("stream: of the pages' device")
     return int(stream.cuda_stream)
+
+
+def _allocating(stream):
+    """New memory belongs to the stream that the call runs on: what another stream freed may still be in use there."""
+    if stream is None:
+        return _NOTHING
+    import torch
+    return torch.cuda.stream(stream)
+
+
+_NOTHING = contextlib.nullcontext()
 
 
 class Cache:
@@ -222,9 +234,8 @@ class Cache:
         need = L.homcomp_cache_attend_scratch(args, t)
         if need:
             if scratch is None:
-                scratch = q.new_empty((need + 3) // 4, dtype=self._float32)
-                if stream is not None:
-                    scratch.record_stream(stream)
+                with _allocating(stream):
+                    scratch = q.new_empty((need + 3) // 4, dtype=self._float32)
             elif scratch.device != self._device or not scratch.is_contiguous():
                 raise ValueError("scratch: contiguous, on the pages' device")
             t = packed(scratch.data_ptr(), scratch.numel() * scratch.element_size())
@@ -249,7 +260,8 @@ class Cache:
         weights               float32 [sequences, kv_heads, at least max_length], as attend gathers them
         first, recent         slots at the front and at the back that stay whatever their weight
         to_table, to_lengths  where the rows go (the table is the caller's, its pages nobody's), and how many there are then
-        to_weights, kept      [sequences, kv_heads, keep] float32 and int32: weights and old slots of the rows that stay
+        to_weights, kept      [sequences, kv_heads, keep] float32 and int32: weights and old slots of the rows that stay; by default new
+                              memory of the call's stream
         """
         args, n, width = self._args(table, lengths)
         at_table = self._ints("to_table", to_table, 2)
@@ -265,11 +277,9 @@ class Cache:
         if stride < max_length:
             raise ValueError(f"weights: [sequences, kv_heads, at least max_length = {max_length}]")
         shape = (n, self.kv_heads, keep)
-        to_weights = weights.new_empty(shape) if to_weights is None else to_weights
-        kept = weights.new_empty(shape, dtype=self._int32) if kept is None else kept
-        if stream is not None:
-            to_weights.record_stream(stream)
-            kept.record_stream(stream)
+        with _allocating(stream):
+            to_weights = weights.new_empty(shape) if to_weights is None else to_weights
+            kept = weights.new_empty(shape, dtype=self._int32) if kept is None else kept
         t = _EVICTION.pack(self._whole("weights", weights, (n, self.kv_heads, stride), self._float32), stride, max_length, keep, first, recent, at_table,
                            to_table.shape[1], self._whole("to_lengths", to_lengths, (n,), self._int32),
                            self._whole("to_weights", to_weights, shape, self._float32), self._whole("kept", kept, shape, self._int32))

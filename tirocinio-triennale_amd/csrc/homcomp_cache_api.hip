@@ -11,7 +11,8 @@
 namespace {
 
 constexpr int64_t kMostSlots = (int64_t)INT32_MAX - 64;
-constexpr int64_t kMostWorkgroups = INT32_MAX;
+constexpr int64_t kMostWorkgroups = UINT32_MAX / 256;   // a launch has fewer than 2^32 threads
+
 constexpr int kComputeUnits = 256;
 
 int launched(hipError_t e)
@@ -78,7 +79,7 @@ int rows_call(bool store, const homcomp_cache *cache, void *k, void *v, int type
     const int rc = cache_args(cache, SIZE_MAX, &c, &nb);
     if (rc) return rc;
     if (!type_ok(type)) return HOMCOMP_ERR_INVALID_ARG;
-    if (n_rows > (size_t)INT32_MAX || ((int64_t)n_rows / 16 + 2 * (int64_t)cache->n_seqs) * cache->kv_heads > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
+    if (n_rows > (size_t)INT32_MAX || ((int64_t)n_rows / 16 + 2 * (int64_t)cache->n_seqs) * cache->kv_heads > 4 * (kMostWorkgroups - 1)) return HOMCOMP_ERR_INVALID_ARG;
     if (c.n_seqs == 0 || n_rows == 0) return HOMCOMP_OK;
     if (!k || !v || !starts) return HOMCOMP_ERR_INVALID_ARG;
     if (!aligned(k, bytes_of(type)) || !aligned(v, bytes_of(type)) || !aligned(starts, 4)) return HOMCOMP_ERR_ALIGNMENT;
@@ -129,8 +130,9 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
     each = (each + hc::kAttendWaves - 1) / hc::kAttendWaves * hc::kAttendWaves;
     p->split_records = (int)each;
     p->splits = (int)((records + each - 1) / each);
-    if (units * p->splits > kMostWorkgroups || (int64_t)c->n_seqs * c->kv_heads * ((most + 31) / 32) > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
-    if (units * hc::kColumns > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
+    // (k_cache_attend, k_cache_join; of k_cache_weights, which takes a few batches for every sequence and head, the batches' number)
+    if (units * p->splits > kMostWorkgroups || units * p->columns > kMostWorkgroups) return HOMCOMP_ERR_INVALID_ARG;
+    if ((int64_t)c->n_seqs * c->kv_heads > kMostWorkgroups / 2 || (int64_t)c->n_seqs * c->kv_heads * ((most + 31) / 32) > INT32_MAX) return HOMCOMP_ERR_INVALID_ARG;
     if (p->splits > 1) {
         const size_t parts = (size_t)units * (size_t)p->splits * hc::kColumns;
         p->partial_bytes = parts * (size_t)(32 * nb) * sizeof(float);
@@ -235,7 +237,8 @@ int homcomp_cache_evict(const homcomp_cache *cache, const homcomp_eviction *t, v
     if (t->keep < 1 || t->keep > (size_t)kMostSlots || t->first > t->keep || t->recent > t->keep - t->first) return HOMCOMP_ERR_INVALID_ARG;
     if (t->to_table_stride > (size_t)kMostSlots / (size_t)cache->page_tokens || t->keep > t->to_table_stride * (size_t)cache->page_tokens)
         return HOMCOMP_ERR_INVALID_ARG;
-    if (t->weight_stride < t->max_length || (int64_t)cache->n_seqs * cache->kv_heads * (int64_t)((t->keep + 31) / 32) > kMostWorkgroups)
+    if (t->weight_stride < t->max_length || (int64_t)cache->n_seqs * cache->kv_heads * (int64_t)((t->keep + 127) / 128) > kMostWorkgroups ||
+        (int64_t)cache->n_seqs * cache->kv_heads > kMostWorkgroups / 4)
         return HOMCOMP_ERR_INVALID_ARG;
     if (a.c.n_seqs == 0) return HOMCOMP_OK;
     if (!t->d_weights || !t->d_to_table || !t->d_to_lengths || !t->d_to_weights || !t->d_kept) return HOMCOMP_ERR_INVALID_ARG;

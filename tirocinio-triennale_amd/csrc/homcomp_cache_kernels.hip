@@ -558,7 +558,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
     r.factor = ldexpf(a.scale * kLog2e, (FORM == kWhole ? -14 : 10) + e);
     const int own = slot0 + row;
     r.see_to = !there ? 0 : (a.causal ? (own + 1 < length ? own + 1 : length) : length);
-    r.see_from = a.window > 0 && own + 1 - a.window > 0 ? own + 1 - a.window : 0;
+    r.see_from = a.window > 0 && own + 1 > a.window ? own + 1 - a.window : 0;
 }
 
 // What a lane holds of a record: rows of the products' operands, and the scales of what it gets back.
@@ -681,7 +681,7 @@ __device__ __forceinline__ void seen_records(const AttendArgs &a, int count, int
     if (last_row >= count) last_row = count - 1;
     int end = length, begin = 0;
     if (a.causal && slot0 + last_row + 1 < end) end = slot0 + last_row + 1;
-    if (a.window > 0 && slot0 + first_row + 1 - a.window > 0) begin = slot0 + first_row + 1 - a.window;
+    if (a.window > 0 && slot0 + first_row + 1 > a.window) begin = slot0 + first_row + 1 - a.window;
     if (end < 0) end = 0;
     *from = begin >> 5;
     *to = begin < end ? (end + 31) >> 5 : begin >> 5;
@@ -703,7 +703,7 @@ __device__ __forceinline__ void seen_by_all(const AttendArgs &a, int count, int 
     int last_row = (tile * COLUMNS + COLUMNS - 1) / a.group;
     if (last_row >= count) last_row = count - 1;
     *to = a.causal && slot0 + first_row + 1 < length ? slot0 + first_row + 1 : length;
-    *from = a.window > 0 && slot0 + last_row + 1 - a.window > 0 ? slot0 + last_row + 1 - a.window : 0;
+    *from = a.window > 0 && slot0 + last_row + 1 > a.window ? slot0 + last_row + 1 - a.window : 0;
 }
 
 // One column's share of a workgroup's result: out rows of 16 columns, 16 threads each.
@@ -1768,7 +1768,7 @@ static hipError_t attend_of(const AttendArgs &a, hipStream_t s)
             e = hipGetLastError();
         }
     }
-    if (e == hipSuccess && a.weights) {
+    if (e == hipSuccess && a.weights && a.c.max_slots > 0) {
         const uint32_t records = ((uint32_t)a.c.max_slots + kRecordSlots - 1) / kRecordSlots;
         const uint32_t all = (records + kAttendWaves * kHeldRecords - 1) / (kAttendWaves * kHeldRecords);   // batches of a sequence and head
         const uint32_t units = (uint32_t)a.c.kv_heads * (uint32_t)a.c.n_seqs;
