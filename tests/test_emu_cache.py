@@ -106,6 +106,13 @@ def test_attend_hard_rows(world, edit, type_):
 
 
 @pytest.mark.parametrize("type_", ["bf16", "f32"])
+@pytest.mark.parametrize("q_scale", [1e20, 1e-25])
+@pytest.mark.parametrize("group", [2, 20])
+def test_attend_large_and_small_queries(world, group, q_scale, type_):
+    check_attend(world, [70], [2], 1, group, 64, 32, type_, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f32"])
 def test_operators_together(world, type_):
     check_run(world, type_=type_)
 

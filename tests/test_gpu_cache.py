@@ -383,6 +383,13 @@ def test_queries_that_are_none(world, type_, group):
     check_attend(world, [90, 40], [2, 2], 1, group, 64, 32, type_, q_edit=edit)
 
 
+@pytest.mark.parametrize("type_", ["bf16", "f32"])
+@pytest.mark.parametrize("q_scale", [1e20, 1e-25])
+@pytest.mark.parametrize("group", [2, 20])
+def test_attend_large_and_small_queries(world, group, q_scale, type_):
+    check_attend(world, [70, 300], [2, 1], 1, group, 128, 32, type_, q_scale=q_scale)
+
+
 def test_memory_for_a_stream_comes_from_it(world):
     """Scratch memory and results that a call makes for another stream are that stream's."""
     seen = []

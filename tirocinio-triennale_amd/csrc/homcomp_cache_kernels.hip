@@ -896,10 +896,13 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
         }
     }
     for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
-    if (__builtin_amdgcn_ballot_w64(most > 15.0f) != 0) {
+    if (__builtin_amdgcn_ballot_w64(most > 15.0f || !(fabsf(bias) < 0x1p16f)) != 0) {
+        float e[8];   // (rounded before the reference is taken off: with exponents above 2^16 the product's rounding would count)
         most = kNegInf;
-        for (int i = 0; i < 8; ++i)
-            if (seen >> i & 1) most = fmaxf(most, x[i >> 2][i & 3] * q.factor);
+        for (int i = 0; i < 8; ++i) {
+            e[i] = x[i >> 2][i & 3] * q.factor;
+            if (seen >> i & 1) most = fmaxf(most, e[i]);
+        }
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
         const float now = fmaxf(s.top, most);
@@ -909,7 +912,7 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
         for (int r = 0; r < 4; ++r)
             for (int i = 0; i < NB / 2; ++i)
                 for (int n = 0; n < 4; ++n) s.o[i][n][r] *= shrink;
-        for (int i = 0; i < 8; ++i) p[i] = (seen >> i & 1) ? fmaf(x[i >> 2][i & 3], q.factor, 7.0f - now) : kNegInf;
+        for (int i = 0; i < 8; ++i) p[i] = (seen >> i & 1) ? e[i] - now + 7.0f : kNegInf;
     }
     for (int i = 0; i < 8; ++i) {
         p[i] = __builtin_amdgcn_exp2f(p[i]);
