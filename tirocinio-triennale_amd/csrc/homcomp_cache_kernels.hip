@@ -281,6 +281,8 @@ __device__ __forceinline__ void wave_lds_order()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// What bounds it is quantising, 1500 vector instructions for sixteen slots of 128 values: 123 thousand slots and heads take 29 us, 2.8 TB/s of rows
+// and records.  (36 with neighbours exchanged through LDS and borders looked at value by value.)
 // Keys: four lanes to a slot, a lane's eight values of every block.  Values' codes of a slot lie two bytes at a time among those of seven others: the
 // wave gathers eight slots' words in LDS and writes them whole, except where not all eight are its own.
 template <int NB, int TY>
@@ -459,9 +461,15 @@ __global__ __launch_bounds__(256) void k_cache_load(CacheArgs c, RowsArgs a, uin
 //            parts where q is 32 bits wide.  The lo part is one more product over (block, part of the sums of q).
 //   values   O[value, column] = sum_slots c[slot, value] (p s_b)[slot, column] + (sum_slots lo_b p)
 //            p s_b is rounded to bfloat16 (two or three parts for outputs of 16 and 32 bits' precision); p carries 2^64 so that
-//            products with codes of 2^-133 stay normal numbers.
+//            products with codes of 2^-133 stay normal numbers.  For 16-bit outputs a record whose values all fit float16 is multiplied as
+//            float16 numbers lo + s c instead: a third of the vector instructions.
 // A wave's two products of 16 slots each take the slots so that what lane group g gets as scores (rows 4 g + r of both) is
 // exactly what it owes the values' product as operand (slots 8 g .. 8 g + 7): nothing is exchanged between lanes.
+//
+// What bounds it is reading the records.  64 sequences of up to 8192 slots, 8 heads of 128 values, four columns each: 327 MB in 83 us, 3.9 TB/s, vector
+// instructions busy for 40 % of it (330 for a record); joining the parts adds 6 us.  One sequence of 131072
+// slots: 168 MB in 34 us, 4.9 TB/s, what a copy of the same bytes reaches.  Values as codes: 106 and 47 us.  Records through LDS
+// one ahead, from where operands are taken: without it (operands loaded from memory in their order) 236 us for the batch.
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -INFINITY;
 
@@ -844,8 +852,10 @@ __device__ __forceinline__ void values_by_numbers(const uint8_t *at, const uint8
         for (int n = 0; n < 2; ++n) {
             u32x4 v;
             for (int i = 0; i < 4; ++i) {
-                const uint32_t word = (b & 1) ? codes[i] >> 8 : codes[i], sw = step[i], lw = low[i];   // (a cast of an element in place takes the vector's first one)
-                v[i] = __builtin_bit_cast(uint32_t, fma_pair(n ? codes_at_4(word, under) : codes_at_0(word, under), __builtin_bit_cast(f16x2, sw), __builtin_bit_cast(f16x2, lw)));
+                // (copies: a cast of an element in place takes the vector's first one)
+                const uint32_t word = (b & 1) ? codes[i] >> 8 : codes[i], sw = step[i], lw = low[i];
+                const f16x2 c = n ? codes_at_4(word, under) : codes_at_0(word, under);
+                v[i] = __builtin_bit_cast(uint32_t, fma_pair(c, __builtin_bit_cast(f16x2, sw), __builtin_bit_cast(f16x2, lw)));
             }
             f32x4 &o = s.o[b >> 1][2 * (b & 1) + n];
             for (int e = 0; e < NP; ++e) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v), w[e], o, 0, 0, 0);
@@ -856,7 +866,8 @@ __device__ __forceinline__ void values_by_numbers(const uint8_t *at, const uint8
 // One record.  A new reference exponent costs a multiplication of everything gathered, so it is taken only where a weight
 // would exceed 2^8 (32-bit sums have room for that); a lane looks at its own eight slots alone, and lanes exchange only then.
 template <int NB, int TY, bool FINE>
-__device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, query_parts<TY>()> &q, int lane, int slot0, int length, bool masked, const f32x4 &zero, const Under &under, Gathered<NB> &s)
+__device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, query_parts<TY>()> &q, int lane, int slot0, int length, bool masked,
+                                              const f32x4 &zero, const Under &under, Gathered<NB> &s)
 {
     constexpr int NQ = query_parts<TY>();
     f32x4 x[2];
@@ -941,7 +952,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     float (*s_o)[kColumns][D + 4] = (float (*)[kColumns][D + 4])s_mem;
     __shared__ float s_top[kAttendWaves][kColumns], s_total[kAttendWaves][kColumns];
     // parts outermost: workgroups go to the eight dies in turn, and later parts are the ones that shorter sequences lack (parts
-    // innermost: half of the compute units idle on a batch of lengths from a tenth to all of 8192, 144 us instead of 92)
+    // innermost: half of the compute units idle on a batch of lengths from a tenth to all of 8192, 144 us when this order took 109)
     const uint32_t units = gridDim.x / (unsigned)a.splits;
     const int split = (int)(blockIdx.x / units);
     const uint32_t unit = blockIdx.x % units;    // (sequence, head, tile)
@@ -1042,7 +1053,11 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
 //
 // Vector and matrix instructions about balance: for a record and 16 columns 8 multiply-adds, 8 exponentials (four times the cost
 // of others) and 25 more against 24 products of 16 cycles.  (With whole codes as keys, their scores scaled in 32 bits as above, it was 64 more
-// vector instructions for 8 products less, and 1410 us instead of what the table says for 2 x 2048 rows over 10007 slots.)
+// vector instructions for 8 products less, and 1410 us instead of 1190.)
+//
+// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1190 us, 510 TFLOP/s of the two products (603 GFLOP). The matrix unit
+// is busy 30 % of it (a third of that with the keys' second parts), vector instructions 43 %, LDS 21 %; two waves for each SIMD, which
+// a barrier for every two records keeps in step, do not put them beside each other fully.  Keys in one part: 960 us, but lse off by 1e-4.
 template <int NB>
 struct WideRecord {
     static constexpr uint32_t kRest = 2048u * NB, kValues = 4096u * NB, kBytes = 6144u * NB;   // keys from 0, their second parts
@@ -1564,6 +1579,7 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t *sums, 
 // A workgroup per sequence and head.  A thread holds sixteen neighbouring weights, so that ranks need one prefix sum over the threads; sequences
 // of up to 16384 slots are read once, longer ones once for each of the passes.  The key of the last weight to stay is found 11,
 // 11 and 10 bits at a time from the top: counts in LDS, then a prefix sum from the largest bin down.
+// Bound by the passes' barriers and instructions, not by memory: 128 heads of up to 16384 slots take 16 us, 8 of 1100 slots 10.
 __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
 {
     __shared__ uint32_t s_bins[kSelectBins];
@@ -1657,6 +1673,8 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
 }
 
 // A wave moves the kept rows into one record of the new pages: where each comes from is found once and handed out through LDS.
+// Values' codes of a slot lie two bytes at a time among those of its seven neighbours, so that nearly all lines of the old records are read:
+// 4096 kept of up to 16384 slots, 16 sequences of 8 heads of 128 values, 82 MB, take 40 us.
 template <int NB>
 __global__ __launch_bounds__(256) void k_cache_move(EvictArgs a, int records)
 {
