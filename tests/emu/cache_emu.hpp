@@ -67,6 +67,7 @@ inline T emu_shfl(unsigned site, T v, int src)
 #define __shfl(v, src, width) emu_shfl(__LINE__, v, src)
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_logf(x) log2f(x)
+#define __builtin_amdgcn_sched_barrier(x) ((void)0)
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define __builtin_amdgcn_fractf(x) ((x) - floorf(x))
 inline uint32_t atomicAdd(uint32_t *p, uint32_t v) { return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST); }

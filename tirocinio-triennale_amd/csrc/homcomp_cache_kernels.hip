@@ -1053,11 +1053,11 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
 //
 // Vector and matrix instructions about balance: for a record and 16 columns 8 multiply-adds, 8 exponentials (four times the cost
 // of others) and 25 more against 24 products of 16 cycles.  (With whole codes as keys, their scores scaled in 32 bits as above, it was 64 more
-// vector instructions for 8 products less, and 1410 us instead of 1190.)
+// vector instructions for 8 products less, and 1410 us when this took 1190.)
 //
-// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1190 us, 510 TFLOP/s of the two products (603 GFLOP). The matrix unit
-// is busy 30 % of it (a third of that with the keys' second parts), vector instructions 43 %, LDS 21 %; two waves for each SIMD, which
-// a barrier for every two records keeps in step, do not put them beside each other fully.  Keys in one part: 960 us, but lse off by 1e-4.
+// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1070 us, 560 TFLOP/s of the two products (603 GFLOP). The matrix unit
+// is busy 34 % of it (a third of that with the keys' second parts), vector instructions 48 %, LDS 24 %; two waves for each SIMD, which
+// a barrier for every two records keeps in step, do not put them beside each other fully.  Keys in one part: a fifth less, but lse off by 1e-4.
 template <int NB>
 struct WideRecord {
     static constexpr uint32_t kRest = 2048u * NB, kValues = 4096u * NB, kBytes = 6144u * NB;   // keys from 0, their second parts
@@ -1150,16 +1150,24 @@ template <int NB, int CT, int NP>
 __device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB, 1> (&q)[CT], int lane, int slot0, bool masked, const f32x4 &zero, WideGathered<NB> (&s)[CT])
 {
     f32x4 e[CT][2];   // exponents of slots slot0 + 4 T ..
-    for (int b = 0; b < NB; ++b) {
-        f16x8 k[2], rest[2];
-        for (int T = 0; T < 2; ++T) {
-            k[T] = *(const f16x8 *)(at + ((T * NB + b) * 64 + lane) * 16);
-            rest[T] = *(const f16x8 *)(at + WideRecord<NB>::kRest + ((T * NB + b) * 64 + lane) * 16);
-        }
-        for (int T = 0; T < 2; ++T)
-            for (int t = 0; t < CT; ++t) e[t][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest[T], q[t].q[b][0], b ? e[t][T] : zero, 0, 0, 0);
-        for (int T = 0; T < 2; ++T)
-            for (int t = 0; t < CT; ++t) e[t][T] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[T], q[t].q[b][0], e[t][T], 0, 0, 0);
+    // Operands are read kAhead products in front of their own: left to itself the compiler reads each where it is needed, to save registers, and a
+    // wave then waits for LDS in front of every pair of products (1190 us instead of 1070, at 2 x 2048 rows over 10007 slots).
+    constexpr int kAhead = 3;
+    static_assert(4 * NB % (kAhead + 1) == 0, "values follow keys in the ring");
+    f16x8 ring[kAhead + 1];
+    auto read_keys = [&](int n) __attribute__((always_inline)) {   // block n / 4: second parts of both T, then first ones
+        return *(const f16x8 *)(at + ((n & 2) ? 0u : WideRecord<NB>::kRest) + (((n & 1) * NB + (n >> 2)) * 64 + lane) * 16);
+    };
+    auto read_values = [&](int n) __attribute__((always_inline)) { return *(const f16x8 *)(at + WideRecord<NB>::kValues + (n * 64 + lane) * 16); };
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) ring[n] = read_keys(n);
+#pragma unroll
+    for (int n = 0; n < 4 * NB; ++n) {
+        ring[(n + kAhead) % (kAhead + 1)] = n + kAhead < 4 * NB ? read_keys(n + kAhead) : read_values(n + kAhead - 4 * NB);
+        __builtin_amdgcn_sched_barrier(0);
+        for (int t = 0; t < CT; ++t)
+            e[t][n & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[n % (kAhead + 1)], q[t].q[n >> 2][0], n < 2 ? zero : e[t][n & 1], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
     }
     bool higher = false;
     for (int t = 0; t < CT; ++t) {
@@ -1197,12 +1205,14 @@ __device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB,
             if (NP == 2) w[t][NP - 1][i] = (_Float16)(p - (float)w[t][0][i]);
         }
     }
-    for (int i = 0; i < NB / 2; ++i) {
-        for (int n = 0; n < 4; ++n) {
-            const f16x8 v = *(const f16x8 *)(at + WideRecord<NB>::kValues + ((i * 4 + n) * 64 + lane) * 16);
-            for (int t = 0; t < CT; ++t)
-                for (int k = 0; k < NP; ++k) s[t].o[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[t][k], s[t].o[i][n], 0, 0, 0);
-        }
+#pragma unroll
+    for (int n = 0; n < 2 * NB; ++n) {
+        if (n + kAhead < 2 * NB) ring[(n + kAhead) % (kAhead + 1)] = read_values(n + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+        for (int t = 0; t < CT; ++t)
+            for (int k = 0; k < NP; ++k)
+                s[t].o[n >> 2][n & 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[n % (kAhead + 1)], w[t][k], s[t].o[n >> 2][n & 3], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
