@@ -748,8 +748,9 @@ __device__ __forceinline__ int kept_here(int x)
 // (The numbers they stand under are held in registers: one instruction then joins and masks.)
 struct Under {
     uint32_t of_0, of_4;
+    float minus;   // -1, which the compiler would make a conversion and a difference of
 };
-__device__ __forceinline__ Under under_codes() { return {(uint32_t)kept_here(0x64006400), (uint32_t)kept_here(0x54005400)}; }
+__device__ __forceinline__ Under under_codes() { return {(uint32_t)kept_here(0x64006400), (uint32_t)kept_here(0x54005400), __builtin_bit_cast(float, kept_here((int)0xbf800000))}; }
 __device__ __forceinline__ f16x2 codes_at_0(uint32_t w, const Under &u) { return __builtin_bit_cast(f16x2, (w & 0x000f000fu) | u.of_0) - (_Float16)1024.0f; }
 __device__ __forceinline__ f16x2 codes_at_4(uint32_t w, const Under &u) { return __builtin_bit_cast(f16x2, (w & 0x00f000f0u) | u.of_4) - (_Float16)64.0f; }
 __device__ __forceinline__ f16x2 fma_pair(f16x2 a, f16x2 b, f16x2 c) { return __builtin_elementwise_fma(a, b, c); }
@@ -1055,7 +1056,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
 // of others) and 25 more against 24 products of 16 cycles.  (With whole codes as keys, their scores scaled in 32 bits as above, it was 64 more
 // vector instructions for 8 products less, and 1410 us when this took 1190.)
 //
-// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1070 us, 560 TFLOP/s of the two products (603 GFLOP). The matrix unit
+// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1060 us, 570 TFLOP/s of the two products (603 GFLOP). The matrix unit
 // is busy 34 % of it (a third of that with the keys' second parts), vector instructions 48 %, LDS 24 %; two waves for each SIMD, which
 // a barrier for every two records keeps in step, do not put them beside each other fully.  Keys in one part: a fifth less, but lse off by 1e-4.
 template <int NB>
@@ -1108,7 +1109,7 @@ __device__ __forceinline__ bool lay_unit(uint8_t *at, const uint8_t *sides, cons
             for (int i = 0; i < 4; ++i) {
                 const float x = fmaf((float)c[i][0], s, lo), y = fmaf((float)c[i][1], s, lo);
                 const f16x2 k = {(_Float16)x, (_Float16)y};
-                const f16x2 r = {(_Float16)(x - (float)k[0]), (_Float16)(y - (float)k[1])};
+                const f16x2 r = {(_Float16)fmaf((float)k[0], under.minus, x), (_Float16)fmaf((float)k[1], under.minus, y)};   // (exact, one instruction each)
                 first[i] = __builtin_bit_cast(uint32_t, k);
                 rest[i] = __builtin_bit_cast(uint32_t, r);
             }
@@ -1151,7 +1152,7 @@ __device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB,
 {
     f32x4 e[CT][2];   // exponents of slots slot0 + 4 T ..
     // Operands are read kAhead products in front of their own: left to itself the compiler reads each where it is needed, to save registers, and a
-    // wave then waits for LDS in front of every pair of products (1190 us instead of 1070, at 2 x 2048 rows over 10007 slots).
+    // wave then waits for LDS in front of every pair of products (1190 us instead of 1070 then, at 2 x 2048 rows over 10007 slots).
     constexpr int kAhead = 3;
     static_assert(4 * NB % (kAhead + 1) == 0, "values follow keys in the ring");
     f16x8 ring[kAhead + 1];
