@@ -1561,6 +1561,7 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
+typedef float f32x4_of_4 __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kSelectThreads = 1024, kSelectEach = 16, kSelectTile = kSelectThreads * kSelectEach, kSelectBins = 2048;
 // Exclusive prefix of a count per thread over the workgroup.
 __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t *sums, uint32_t *all)
@@ -1611,8 +1612,11 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
     uint32_t key[kSelectEach];
     auto load = [&](int base) __attribute__((always_inline)) {
         const int j = base + tid * kSelectEach;
-        if (j + kSelectEach <= length && ((uintptr_t)(w + j) & 15u) == 0) {
-            load_run<kSelectEach>(w, (uint64_t)j, own);
+        if (j + kSelectEach <= length) {   // (rows of weights lie at multiples of four bytes alone, which is enough for sixteen at once)
+            for (int i = 0; i < kSelectEach / 4; ++i) {
+                const f32x4_of_4 v = *(const f32x4_of_4 *)(w + j + 4 * i);
+                for (int n = 0; n < 4; ++n) own[4 * i + n] = v[n];
+            }
         } else {
             for (int i = 0; i < kSelectEach; ++i) own[i] = j + i < length ? w[j + i] : 0.0f;
         }
