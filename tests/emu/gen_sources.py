@@ -58,9 +58,9 @@ LAUNCHERS = "// ----------------------------------------------------------------
 
 
 def edit(text: str, edits, what: str) -> str:
-    for old, new, *count in edits:
-        if text.count(old) != (count[0] if count else 1):
-            raise SystemExit(f"gen_sources: expected {count[0] if count else 'exactly one'} occurrence(s) in {what} of: {old!r}")
+    for old, new in edits:
+        if text.count(old) != 1:
+            raise SystemExit(f"gen_sources: expected exactly one occurrence in {what} of: {old!r}")
         text = text.replace(old, new)
     for space in ("__attribute__((address_space(3))) ", "__attribute__((address_space(1))) "):
         text = text.replace(space, "")
