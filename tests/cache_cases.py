@@ -1,0 +1,61 @@
+"""Further checks of the 4-bit cache for both places to run it (cache_world.py): calls in which not all is as wide as it could be."""
+import numpy as np
+import torch
+
+import cache_reference as ref
+from cache_world import TYPES, Batch, close
+
+
+def weights_of_rows(q, k, there, rows, n, L, group, scale, causal, window):
+    """The attention that one head's slots receive from rows `rows` (of n) of a sequence of L slots, and how far it may be off: a weight is off
+    by a factor of 1 + 2 e + run + |lse| 2^-22 as cache_reference.attention derives them, the running sum by a rounding for each row."""
+    d = q.shape[-1]
+    w, dw, j = np.zeros(L), np.zeros(L), np.arange(L)
+    for i in rows:
+        at = L - n + i
+        see = there & ((j <= at) if causal else True) & ((j > at - window) if window else True)
+        if not see.any():
+            continue
+        for g in range(group):
+            s = scale * (k[see] @ q[i, g])
+            size = abs(scale) * (np.abs(k[see]) + 2 * np.abs(k[see]).max(-1, keepdims=True)) @ np.abs(q[i, g])
+            z = s.max() + np.log(np.exp(s - s.max()).sum())
+            p = np.exp(s - z)
+            e, run = (64 + d / 32) * 2.0 ** -24 * size.max(), 2.0 ** -20 + L * 2.0 ** -24
+            w[see] += p
+            dw[see] += p * (2 * e + run + abs(z) * 2.0 ** -22) + 2.0 ** -23 * w[see]
+    return w, dw
+
+
+def check_rows_left_out(world, lengths, rows, heads, group, d, page, type_, causal, window, max_rows=None, hold=None, seed=0):
+    """Sequences with more rows than max_rows, or than the arrays hold: the rows that stay get what they get when nothing is left out, the others
+    are left as they were, and weights count the rows that stay."""
+    b = Batch(world, lengths, rows, heads, d, page, seed)
+    b.fill()
+    hold = b.total if hold is None else hold
+    q = torch.from_numpy(b.rng.standard_normal((b.total, heads * group, d)).astype(np.float32)).to(TYPES[type_])
+    out, lse = world.full((hold, heads * group, d), 55.0, TYPES[type_]), world.full((hold, heads * group), 44.0, torch.float32)
+    width = b.table.shape[1] * page
+    weights = world.full((len(lengths), heads, width), 33.0, torch.float32)
+    need = b.c.scratch_bytes(hold, heads * group, len(lengths), b.table.shape[1], TYPES[type_], window=window, weights=True, lse=True, max_rows=max_rows)
+    b.c.attend(world.put(q[:hold]), out, b.d_table, b.d_lengths, b.d_starts, causal=causal, window=window, max_rows=max_rows, lse=lse, weights=weights,
+               scratch=world.full((need // 4 + 4,), float("nan"), torch.float32))
+    held = b.held()
+    keys, vals, there = ([[x[i] for x in per] for per in held] for i in range(3))
+    scale, q = float(np.float32(d ** -0.5)), q.double().numpy()
+    want, want_lse, _, tol, tol_lse, _ = ref.attention(q, keys, vals, there, lengths, b.starts, group, scale, causal, window, type_)
+    got, got_lse, got_w = world.get(out), world.get(lse), world.get(weights)
+    most = hold if max_rows is None else max_rows
+    for s, (L, n) in enumerate(zip(lengths, rows)):
+        first = int(b.starts[s])
+        stay = [i for i in range(n) if i < most and first + i < hold]
+        gone = [first + i for i in range(n) if i not in stay and first + i < hold]
+        at = [first + i for i in stay]
+        close(got_lse[at], want_lse[at], tol_lse[at], f"lse of sequence {s}")
+        close(got[at], want[at], tol[at], f"out of sequence {s}")
+        assert (got[gone] == 55.0).all() and (got_lse[gone] == 44.0).all(), "rows that are left out were written"
+        for h in range(heads):
+            part = q[first:first + n, h * group:(h + 1) * group]
+            w, dw = weights_of_rows(part, keys[s][h], there[s][h], stay, n, L, group, scale, causal, window)
+            close(got_w[s, h, :L], w, dw + 2.0 ** -24 * w, f"weights of sequence {s}")
+        assert (got_w[s, :, L:] == 33.0).all()

@@ -703,6 +703,14 @@ __device__ __forceinline__ int parts_origin(const AttendArgs &a, int count, int 
     else seen_records(a, count, slot0, length, tile, &from, &to);
     return from;
 }
+// Records of a part counted from `origin`.  The host plans parts for window + max_rows slots, which is all that causal rows under a window see.
+// Others see up to the sequence's last slot, and rows that are left out (max_rows, n_rows) stand between: parts are longer then.
+__device__ __forceinline__ int records_of_part(const AttendArgs &a, int length, int origin)
+{
+    if (a.causal || a.window == 0) return a.split_records;
+    const int each = (((length + 31) >> 5) - origin + a.splits - 1) / a.splits;
+    return each <= a.split_records ? a.split_records : (each + kAttendWaves - 1) / kAttendWaves * kAttendWaves;
+}
 // Slots that every one of a tile's columns sees: [*from, *to).
 template <int COLUMNS = kColumns>
 __device__ __forceinline__ void seen_by_all(const AttendArgs &a, int count, int slot0, int length, int tile, int *from, int *to)
@@ -968,10 +976,11 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     int from, to, all_from, all_to;
     seen_records(a, count, slot0, length, tile, &from, &to);
     seen_by_all(a, count, slot0, length, tile, &all_from, &all_to);
-    const int part_from = parts_origin(a, count, slot0, length, tile) + split * a.split_records;
+    const int origin = parts_origin(a, count, slot0, length, tile), part_records = records_of_part(a, length, origin);
+    const int part_from = origin + split * part_records;
     if (split > 0 && part_from >= to) return;   // (one in front of what the tile sees is written all the same, with nothing in it)
     if (from < part_from) from = part_from;
-    if (to > part_from + a.split_records) to = part_from + a.split_records;
+    if (to > part_from + part_records) to = part_from + part_records;
 
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     Queries<NB, NQ> q;
@@ -1239,8 +1248,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
     if (wide * kWide >= count * a.group) return;
     int from, to;
     seen_records(a, count, slot0, length, wide, &from, &to, kWide);
-    from += split * a.split_records;
-    if (to > from + a.split_records) to = from + a.split_records;
+    const int part_records = records_of_part(a, length, from);
+    from += split * part_records;
+    if (to > from + part_records) to = from + part_records;
 
     Queries<NB, 1> q[CT];
     WideGathered<NB> acc[CT];
@@ -1386,7 +1396,8 @@ __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
     if (tile * kColumns + column >= count * a.group) return;
     int from, to;
     seen_records(a, count, slot0, length, tile, &from, &to);
-    int parts = (to - parts_origin(a, count, slot0, length, tile) + a.split_records - 1) / a.split_records;
+    const int origin = parts_origin(a, count, slot0, length, tile), part_records = records_of_part(a, length, origin);
+    int parts = (to - origin + part_records - 1) / part_records;
     if (parts < 1) parts = 1;
     if (parts > a.splits) parts = a.splits;
     const uint64_t at = ((uint64_t)unit * kColumns + (uint32_t)column) * (uint32_t)a.splits;
