@@ -167,6 +167,16 @@ CACHE_EDITS = [
 ]
 
 
+def cache_sources() -> None:
+    os.makedirs(GEN, exist_ok=True)
+    kernels, api, shared = (open(os.path.join(CSRC, f)).read() for f in ("homcomp_cache_kernels.hip", "homcomp_cache_api.hip", "homcomp_cache.hpp"))
+    kernels = edit(kernels, CACHE_EDITS, "homcomp_cache_kernels.hip")
+    api = edit(api, [('#include "../../include/homcomp_cache.h"', '#include "homcomp_cache.h"')], "homcomp_cache_api.hip")
+    api += "namespace hc { void note_hip_error(int) {} }\n"   # (the library's own is in homcomp_api.hip)
+    for name, text in (("homcomp_cache_kernels.cpp", kernels), ("homcomp_cache_api.cpp", api), ("homcomp_cache.hpp", shared)):
+        open(os.path.join(GEN, name), "w").write(text)
+
+
 def build_cache_library(force: bool = False) -> str:
     """The 4-bit cache's entry points and kernels built for the host against the execution model (with the model's allocator)."""
     import subprocess
@@ -175,17 +185,29 @@ def build_cache_library(force: bool = False) -> str:
     inputs += [os.path.join(HERE, f) for f in ("amdgcn_emu.hpp", "cache_emu.hpp", "emu_runtime.hpp", "emu_library.cpp", "gen_sources.py")]
     if not force and os.path.exists(CACHE_LIBRARY) and all(os.path.getmtime(f) <= os.path.getmtime(CACHE_LIBRARY) for f in inputs):
         return CACHE_LIBRARY
-    os.makedirs(GEN, exist_ok=True)
-    kernels, api, shared = (open(os.path.join(CSRC, f)).read() for f in ("homcomp_cache_kernels.hip", "homcomp_cache_api.hip", "homcomp_cache.hpp"))
-    kernels = edit(kernels, CACHE_EDITS, "homcomp_cache_kernels.hip")
-    api = edit(api, [('#include "../../include/homcomp_cache.h"', '#include "homcomp_cache.h"')], "homcomp_cache_api.hip")
-    api += "namespace hc { void note_hip_error(int) {} }\n"   # (the library's own is in homcomp_api.hip)
-    for name, text in (("homcomp_cache_kernels.cpp", kernels), ("homcomp_cache_api.cpp", api), ("homcomp_cache.hpp", shared)):
-        open(os.path.join(GEN, name), "w").write(text)
+    cache_sources()
     subprocess.run([CLANG, *CXXFLAGS, "-O1", "-mf16c", "-mfma", "-ffp-contract=off", "-fPIC", "-shared", "-x", "c++", "-I" + HERE, "-I" + GEN, "-I" + INCLUDE,
                     "-include", os.path.join(HERE, "emu_library_config.h"), "-o", CACHE_LIBRARY, os.path.join(HERE, "emu_library.cpp"),
                     os.path.join(GEN, "homcomp_cache_kernels.cpp"), os.path.join(GEN, "homcomp_cache_api.cpp")], check=True)
     return CACHE_LIBRARY
+
+
+CACHE_LIMITS = os.path.join(GEN, "cache_limits")
+
+
+def build_cache_limits(force: bool = False) -> str:
+    """The cache's kernels at the largest lengths, a workgroup at a time (cache_limits.cpp); returns the program's path."""
+    import subprocess
+
+    source = os.path.join(HERE, "cache_limits.cpp")
+    inputs = [source] + [os.path.join(CSRC, f) for f in CACHE_FILES] + [os.path.join(HERE, f) for f in ("amdgcn_emu.hpp", "cache_emu.hpp", "emu_runtime.hpp", "gen_sources.py")]
+    if not force and os.path.exists(CACHE_LIMITS) and all(os.path.getmtime(f) <= os.path.getmtime(CACHE_LIMITS) for f in inputs):
+        return CACHE_LIMITS
+    cache_sources()
+    subprocess.run([CLANG, *CXXFLAGS, "-O1", "-mf16c", "-mfma", "-ffp-contract=off", "-fsanitize=signed-integer-overflow", "-fsanitize-trap=all",
+                    "-I" + HERE, "-I" + GEN, "-I" + INCLUDE, "-include",
+                    os.path.join(HERE, "emu_library_config.h"), "-o", CACHE_LIMITS, source], check=True)
+    return CACHE_LIMITS
 
 
 PROGRAMS = ("shim_roundtrip", "ring_allreduce", "homcomp_eval")

@@ -1488,7 +1488,9 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
     const Rows rows = rows_of(a.starts, s, a.n_rows);
     const int first = rows.first, count = rows.count < a.max_rows ? rows.count : a.max_rows;
     const int length = sequence_length(a.c, s), slot0 = length - rows.behind;   // slot of the first row (in front of 0: more rows than slots)
-    const int own = 8 * g + 4 * (n & 1) + (n & 2) + ((n >> 2) & 1);   // the lane's slot of a record's weights
+    const uint32_t own = (uint32_t)(8 * g + 4 * (n & 1) + (n & 2) + ((n >> 2) & 1));   // the lane's slot of a record's weights
+    // (records are counted, not slots: the last batch may reach past the last slot, and with it past 2^31)
+    const int held = (int)(((uint32_t)length + 31) >> 5);
     const uint64_t line = ((uint64_t)s * a.c.kv_heads + h) * a.weight_stride;
     RawKeys<NB> raw[kHeldRecords];
     float before[kHeldRecords];
@@ -1496,21 +1498,21 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
     auto load_batch = [&](int it0) __attribute__((always_inline)) {
         coming = 0;
         for (int k = 0; k < kHeldRecords; ++k) {
-            const uint8_t *rec = (it0 + k) * kRecordSlots < length ? record_of(a.c, a.c.table, a.c.table_stride, s, h, (it0 + k) * kRecordSlots, NB) : nullptr;
+            const uint8_t *rec = it0 + k < held ? record_of(a.c, a.c.table, a.c.table_stride, s, h, (it0 + k) * kRecordSlots, NB) : nullptr;
             if (!rec) continue;
             coming |= 1u << k;
             load_raw_keys<NB>(rec, lane, raw[k]);
         }
         for (int k = 0; k < kHeldRecords; ++k) {
-            const int slot = (it0 + k) * kRecordSlots + own;
-            before[k] = a.prior && n < 8 && slot < length ? a.prior[line + (uint64_t)slot] : 0.0f;
+            const uint32_t slot = (uint32_t)(it0 + k) * kRecordSlots + own;
+            before[k] = a.prior && n < 8 && slot < (uint32_t)length ? a.prior[line + (uint64_t)slot] : 0.0f;
         }
     };
     load_batch(begin);
     int tile = -1;
     Queries<NB, NQ> q;
     float lse = 0.0f;
-    for (int it0 = begin; it0 < begin + kBatch * batches && it0 * kRecordSlots < length; it0 += kBatch) {
+    for (int it0 = begin; it0 < begin + kBatch * batches && it0 < held; it0 += kBatch) {
         // the columns of the next tile that sees any of the records (a single tile stays)
         int next = -1;
         auto next_tile = [&]() __attribute__((always_inline)) {
@@ -1555,8 +1557,8 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
         }
         for (int k = 0; k < kHeldRecords; ++k) {
             const float all = sum_over_row(sum[k], n);
-            const int slot = (it0 + k) * kRecordSlots + own;
-            if (n < 8 && slot < length) a.weights[line + (uint64_t)slot] = prior[k] + all;
+            const uint32_t slot = (uint32_t)(it0 + k) * kRecordSlots + own;
+            if (n < 8 && slot < (uint32_t)length) a.weights[line + (uint64_t)slot] = prior[k] + all;
         }
         wave_lds_order();
     }
