@@ -1611,20 +1611,21 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
     __shared__ uint32_t s_sums[kSelectThreads / 64];
     __shared__ uint32_t s_found[2];
     const int h = (int)(blockIdx.x % (unsigned)a.c.kv_heads), s = (int)(blockIdx.x / (unsigned)a.c.kv_heads);
-    const int length = sequence_length(a.c, s), tid = threadIdx.x;
+    // (slots without a sign: tiles reach past the last slot, and with it past 2^31)
+    const uint32_t length = (uint32_t)sequence_length(a.c, s), tid = threadIdx.x, keep = (uint32_t)a.keep;
     const uint64_t unit = (uint64_t)s * a.c.kv_heads + h;
     const float *w = a.weights + unit * a.weight_stride;
-    const int count = length < a.keep ? length : a.keep;
-    const bool all = length <= a.keep;
+    const uint32_t count = length < keep ? length : keep;
+    const bool all = length <= keep;
     uint32_t need = (uint32_t)(a.keep - a.first - a.recent);     // of the candidates, low <= slot < high, to stay
     const bool some = !all && need > 0, once = length <= kSelectTile;
-    const int low = all ? length : a.first, high = all ? length : length - a.recent;
+    const uint32_t low = all ? length : (uint32_t)a.first, high = all ? length : length - (uint32_t)a.recent;
     // a key that is above all weights' for slots that stay anyway, and (not looked at) behind the last
     constexpr uint32_t kStays = 0xffffffffu;
     float own[kSelectEach];
     uint32_t key[kSelectEach];
-    auto load = [&](int base) __attribute__((always_inline)) {
-        const int j = base + tid * kSelectEach;
+    auto load = [&](uint32_t base) __attribute__((always_inline)) {
+        const uint32_t j = base + tid * kSelectEach;
         if (j + kSelectEach <= length) {   // (rows of weights lie at multiples of four bytes alone, which is enough for sixteen at once)
             for (int i = 0; i < kSelectEach / 4; ++i) {
                 const f32x4_of_4 v = *(const f32x4_of_4 *)(w + j + 4 * i);
@@ -1636,7 +1637,7 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
         for (int i = 0; i < kSelectEach; ++i) key[i] = j + i >= low && j + i < high ? weight_key(own[i]) : kStays;
     };
     // (waves that hold nothing go from barrier to barrier)
-    const int wave_first = __builtin_amdgcn_readfirstlane(tid & ~63) * kSelectEach;
+    const uint32_t wave_first = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid & ~63u)) * kSelectEach;
     load(0);
     uint32_t prefix = some ? 0 : kStays - 1, mask = 0;
     if (some) {
@@ -1646,14 +1647,14 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
             s_bins[tid] = 0;
             s_bins[tid + kSelectThreads] = 0;
             __syncthreads();
-            for (int base = 0; base < length; base += kSelectTile) {
+            for (uint32_t base = 0; base < length; base += kSelectTile) {
                 if (!once) load(base);
                 if (base + wave_first >= length) continue;
                 for (int i = 0; i < kSelectEach; ++i)
                     if (key[i] != kStays && (key[i] & mask) == prefix) atomicAdd(&s_bins[(key[i] >> shift) & digits], 1u);
             }
             __syncthreads();
-            const uint32_t bin = (uint32_t)(kSelectBins - 1 - 2 * tid), c0 = s_bins[bin], c1 = s_bins[bin - 1];
+            const uint32_t bin = kSelectBins - 1 - 2 * tid, c0 = s_bins[bin], c1 = s_bins[bin - 1];
             uint32_t total;
             const uint32_t before = block_prefix(c0 + c1, s_sums, &total);
             if (before < need && need <= before + c0 + c1) {
@@ -1669,9 +1670,10 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
     }
     // all with a larger key than `prefix` stay, and `need` of those with that key, the ones in front
     uint32_t greater = 0, equal = 0;   // in front of a tile
-    for (int base = 0; base < length; base += kSelectTile) {
+    for (uint32_t base = 0; base < length; base += kSelectTile) {
         if (!once) load(base);
-        const int j0 = base + tid * kSelectEach, held = length - j0;
+        const uint32_t j0 = base + tid * kSelectEach;
+        const int held = (int)(length - j0);   // (of this thread, none where it is not above 0)
         uint32_t more = 0, same = 0, total;
         for (int i = 0; i < kSelectEach; ++i) {
             more |= key[i] > prefix ? 1u << i : 0u;
@@ -1685,19 +1687,19 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
         if (base + wave_first >= length) continue;
         for (int i = 0; i < kSelectEach; ++i) {
             const bool tied = (same >> i) & 1u;
-            if ((((more >> i) & 1u) || (tied && rank < need)) && at < (uint32_t)count) {
-                a.kept[unit * a.keep + at] = j0 + i;
-                a.to_weights[unit * a.keep + at] = own[i];
+            if ((((more >> i) & 1u) || (tied && rank < need)) && at < count) {
+                a.kept[unit * keep + at] = (int32_t)(j0 + (uint32_t)i);
+                a.to_weights[unit * keep + at] = own[i];
                 ++at;
             }
             rank += tied ? 1u : 0u;
         }
     }
-    for (int i = count + tid; i < a.keep; i += kSelectThreads) {
-        a.kept[unit * a.keep + i] = -1;
-        a.to_weights[unit * a.keep + i] = 0.0f;
+    for (int i = (int)(count + tid); i < a.keep; i += kSelectThreads) {
+        a.kept[unit * keep + i] = -1;
+        a.to_weights[unit * keep + i] = 0.0f;
     }
-    if (h == 0 && tid == 0) a.to_lengths[s] = count;
+    if (h == 0 && tid == 0) a.to_lengths[s] = (int32_t)count;
 }
 
 // A wave moves the kept rows into one record of the new pages: where each comes from is found once and handed out through LDS.
