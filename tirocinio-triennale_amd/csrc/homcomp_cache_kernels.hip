@@ -1695,7 +1695,7 @@ __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
             rank += tied ? 1u : 0u;
         }
     }
-    for (int i = (int)(count + tid); i < a.keep; i += kSelectThreads) {
+    for (uint32_t i = count + tid; i < keep; i += kSelectThreads) {
         a.kept[unit * keep + i] = -1;
         a.to_weights[unit * keep + i] = 0.0f;
     }
@@ -1716,8 +1716,8 @@ __global__ __launch_bounds__(256) void k_cache_move(EvictArgs a, int records)
     const int h = (int)(blockIdx.x / groups % (unsigned)a.c.kv_heads);
     const int s = (int)(blockIdx.x / groups / (unsigned)a.c.kv_heads);
     const int length = sequence_length(a.c, s), count = length < a.keep ? length : a.keep;
+    if (it >= (int)(((uint32_t)count + 31) >> 5)) return;   // (records: slots behind the last one may pass 2^31)
     const int left = count - it * kRecordSlots < kRecordSlots ? count - it * kRecordSlots : kRecordSlots;     // rows of this record
-    if (left <= 0) return;
     uint8_t *to = record_of(a.c, a.to_table, a.to_table_stride, s, h, it * kRecordSlots, NB);
     if (!to) return;
     if (lane < left) {
