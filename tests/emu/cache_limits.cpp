@@ -3,6 +3,7 @@
 //   cache_limits weights    the last workgroup of k_cache_weights, whose batches reach past the last record
 //   cache_limits select     k_cache_select over a whole sequence
 //   cache_limits keep       k_cache_select with almost as many rows to keep, of few
+//   cache_limits columns    k_cache_attend_rows, with waves whose columns are not there
 #define EMU_DEFINE_GLOBALS
 #include "hip/hip_runtime.h"
 
@@ -65,6 +66,34 @@ int main(int argc, char **argv)
         if ((int64_t)groups * 8 * batches < (1 << 26)) return fail("the last workgroup does not reach past 2^26 records");
         if (!emu_run_grid([=]() { blockIdx.x = groups - 1; hc::k_cache_weights<2, 0>(a, records, batches); }, dim3(1), dim3(256))) return fail("weights");
         return a.weights[most - 1] == 0.0f ? 0 : fail("the last weight was not written");
+    }
+    if (what == "columns") {
+        hc::AttendArgs a;
+        memset(&a, 0, sizeof a);
+        a.c = c;
+        a.c.table = (const int32_t *)repeated((size_t)stride * 4);
+        a.c.lengths = numbers({most});
+        a.starts = numbers({0, 17});
+        a.n_rows = a.max_rows = 17;
+        a.group = 1;
+        a.tiles = 2;
+        a.splits = 1;
+        a.split_records = 4;
+        a.window = 40;
+        a.causal = 1;
+        a.wide_tiles = 1;
+        a.tiles_in_wide = 16;
+        a.q_row_stride = a.out_row_stride = 64;
+        a.q_head_stride = a.out_head_stride = 64;
+        a.scale = 1.0f;
+        a.q = emu_device_alloc_named(17 * 128, "q", 16);
+        a.out = emu_device_alloc_named(17 * 128, "out", 16);
+        a.left_over = (uint32_t *)numbers({7});
+        memset(a.out, 0x55, 17 * 128);
+        if (!emu_run_grid([=]() { hc::k_cache_attend_rows<2, 0, 8, 2>(a); }, dim3(1), dim3(512))) return fail("columns");
+        for (int i = 0; i < 17 * 64; ++i)
+            if (((uint16_t *)a.out)[i] != 0) return fail("rows that see no page");
+        return a.left_over[0] == 0 ? 0 : fail("columns left over");
     }
     hc::EvictArgs e;
     memset(&e, 0, sizeof e);

@@ -5,7 +5,7 @@ import subprocess
 import pytest
 
 
-@pytest.mark.parametrize("what", ["weights", "select", "keep"])
+@pytest.mark.parametrize("what", ["weights", "select", "keep", "columns"])
 def test_near_2_to_31_slots(emu_sources, what):
     r = subprocess.run([emu_sources.build_cache_limits(), what], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr

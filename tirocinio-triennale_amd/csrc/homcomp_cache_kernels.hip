@@ -1255,10 +1255,11 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
     Queries<NB, 1> q[CT];
     WideGathered<NB> acc[CT];
     const int wave_tile = wide * W + wave;   // of 16 CT columns
-    int own_from, own_to, all_from, all_to;
-    seen_records(a, count, slot0, length, wave_tile, &own_from, &own_to, kColumns * CT);
-    seen_by_all<kColumns * CT>(a, count, slot0, length, wave_tile, &all_from, &all_to);
-    if (wave_tile * kColumns * CT >= count * a.group) own_to = own_from;
+    int own_from = 0, own_to = 0, all_from = 0, all_to = 0;   // (nothing, where the wave's columns are not there)
+    if (wave_tile * kColumns * CT < count * a.group) {
+        seen_records(a, count, slot0, length, wave_tile, &own_from, &own_to, kColumns * CT);
+        seen_by_all<kColumns * CT>(a, count, slot0, length, wave_tile, &all_from, &all_to);
+    }
     for (int t = 0; t < CT; ++t) {
         load_queries<NB, TY, kWhole>(a, h, first, count, slot0, length, (wave_tile * CT + t) * kColumns + n, g, q[t]);
         acc[t].top = kNegInf;
