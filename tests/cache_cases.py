@@ -59,3 +59,33 @@ def check_rows_left_out(world, lengths, rows, heads, group, d, page, type_, caus
             w, dw = weights_of_rows(part, keys[s][h], there[s][h], stay, n, L, group, scale, causal, window)
             close(got_w[s, h, :L], w, dw + 2.0 ** -24 * w, f"weights of sequence {s}")
         assert (got_w[s, :, L:] == 33.0).all()
+
+
+# Constant blocks far from the others: held exactly (s = 0) up to bfloat16's largest number.
+LARGEST = float(torch.tensor(0x7f7f, dtype=torch.int16).view(torch.bfloat16))
+
+
+def far_values(k, v, slots):
+    v[slots % 5 == 2] = 2.0 ** 66
+
+
+def farthest_values(k, v, slots):
+    v[slots % 7 == 3] = float(torch.tensor(1e38).bfloat16())
+    v[slots % 32 == 9] = -LARGEST
+
+
+def only_farthest_values(k, v, slots):
+    v[:] = LARGEST
+
+
+def last_value_far(k, v, slots):
+    """Seen by the last row of a causal batch alone, or the last columns."""
+    v[slots == slots.max()] = LARGEST
+
+
+def far_and_tiny_values(k, v, slots):
+    v[slots % 11 == 4] = 2.0 ** 41
+    v[slots % 3 == 0] = 2.0 ** -40
+
+
+FAR = [far_values, farthest_values, only_farthest_values, last_value_far, far_and_tiny_values]

@@ -1,7 +1,8 @@
 """Further cases of the 4-bit cache on the CPU execution model."""
 import pytest
 
-from cache_cases import check_rows_left_out
+from cache_cases import FAR, check_rows_left_out
+from cache_world import check_attend
 from test_emu_cache import _release, world  # noqa: F401
 
 # sequences' rows, max_rows, rows the arrays hold
@@ -13,3 +14,14 @@ LEFT_OUT = [([300], 5, None), ([300], None, 8), ([300, 3], 2, 302)]
 @pytest.mark.parametrize("group,type_", [(1, "f32"), (1, "bf16"), (9, "bf16")])   # (the last: many columns)
 def test_rows_left_out(world, rows, max_rows, hold, causal, window, group, type_):  # noqa: F811
     check_rows_left_out(world, [400, 40][:len(rows)], rows, 1, group, 64, 32, type_, causal, window, max_rows, hold)
+
+
+# (float16 results do not reach that far)
+@pytest.mark.parametrize("edit", FAR)
+@pytest.mark.parametrize("lengths,rows,group,d,type_,kw", [
+    ([70], [2], 2, 64, "f32", {}), ([70], [2], 2, 64, "bf16", {}),
+    ([300], [1], 1, 128, "f32", {}), ([300], [1], 1, 128, "bf16", dict(weights=True)),     # parts joined
+    ([100], [9], 3, 64, "bf16", {}), ([100], [9], 3, 64, "bf16", dict(causal=False, window=20)),   # many columns
+])
+def test_attend_far_values(world, edit, lengths, rows, group, d, type_, kw):  # noqa: F811
+    check_attend(world, lengths, rows, 1, group, d, 32, type_, edit=edit, **kw)

@@ -1,7 +1,8 @@
 """Further cases of the 4-bit cache on the GPU."""
 import pytest
 
-from cache_cases import check_rows_left_out
+from cache_cases import FAR, check_rows_left_out
+from cache_world import check_attend
 from test_emu_cache_cases import LEFT_OUT
 from test_gpu_cache import world  # noqa: F401
 
@@ -13,3 +14,13 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("group,d,type_", [(1, 64, "f32"), (4, 128, "f16"), (9, 64, "bf16"), (20, 256, "bf16")])
 def test_rows_left_out(world, rows, max_rows, hold, causal, window, group, d, type_):  # noqa: F811
     check_rows_left_out(world, [1300, 40][:len(rows)], rows, 1, group, d, 32, type_, causal, window, max_rows, hold)
+
+
+@pytest.mark.parametrize("edit", FAR)
+@pytest.mark.parametrize("lengths,rows,group,d,type_,kw", [
+    ([70], [2], 2, 64, "f32", {}), ([70], [2], 2, 256, "bf16", {}),
+    ([1300, 64], [1, 1], 1, 128, "f32", {}), ([1300], [1], 1, 128, "bf16", dict(weights=True)),         # parts joined
+    ([200], [9], 3, 128, "bf16", {}), ([200, 90], [40, 3], 3, 64, "bf16", dict(causal=False, window=20)),   # many columns
+])
+def test_attend_far_values(world, edit, lengths, rows, group, d, type_, kw):  # noqa: F811
+    check_attend(world, lengths, rows, 1, group, d, 32, type_, edit=edit, **kw)

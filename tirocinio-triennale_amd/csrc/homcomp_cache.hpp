@@ -49,7 +49,7 @@ struct AttendArgs {
     int32_t causal, window;     // window 0: none
     float scale;
     float *lse;                 // null: not wanted
-    float *partial;             // of more than one split: [tile][kColumns][split][head_dim]
+    float *partial;             // of more than one split: [tile][kColumns][split][head_dim], means
     float *partial_sums;        // [tile][kColumns][split][2]: exponent the part is relative to, sum
     int32_t columns;            // columns that a tile can have
     int32_t wide_tiles;         // tiles of many columns that a sequence's rows can take, 0: not that kernel

@@ -722,17 +722,15 @@ __device__ __forceinline__ void seen_by_all(const AttendArgs &a, int count, int 
     *from = a.window > 0 && slot0 + last_row + 1 > a.window ? slot0 + last_row + 1 - a.window : 0;
 }
 
-// One column's share of a workgroup's result: out rows of 16 columns, 16 threads each.
+// One column's share of a workgroup's result: out rows of 16 columns, 16 threads each.  o: the mean of the values; total: the sum of the weights,
+// relative to 2^top.
 template <int NB, int TY>
 __device__ __forceinline__ void write_result(const AttendArgs &a, int h, int first, int column, int part, float top, float total, const float *o)
 {
     const int row = column / a.group, head = column - row * a.group;
     constexpr int N = 2 * NB;   // values of this thread: part * N ..
-    float x[N];
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    for (int i = 0; i < N; ++i) x[i] = total == 0.0f ? 0.0f : o[i] * inv;
     const uint64_t at = (uint64_t)(first + row) * a.out_row_stride + (uint64_t)(h * a.group + head) * a.out_head_stride + (uint64_t)(part * N);
-    store_run<N, TY>(a.out, at, x);
+    store_run<N, TY>(a.out, at, o);
     if (a.lse && part == 0)
         a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)] =
             total == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(total)) * kLn2;
@@ -775,12 +773,15 @@ struct Gathered {
     f32x4 o[NB / 2][4];   // sum of value * p, values 64 i + 16 p + 4 g + r, times 2^7
     float top;            // exponent p is relative to; at most 8 below the largest so far
     float total;          // sum of the lane's p, times 2^7
+    uint32_t far;         // 1: a value of 2^40 or more was among them, o is times 2^-48 more (the same in all lanes)
 };
 
 // The values' product in exact codes, for any values: p s_b in NP parts of bfloat16 against the codes.
 // Codes count from the middle, c - 8 in even slots and c - 7 in odd ones (numbers of the codes' own form; on the average the
 // middle itself), the rest is lo + 8 s or lo + 7 s: with codes from 0 the two sums would grow with the number of slots and nearly
 // cancel where a block's values lie around zero, each with roundings of its own.
+// A block's lowest number can be as large as a bfloat16.  From 2^40 on p goes to its product small instead of large, and all that is gathered
+// is held 2^-48 times: room for 2^31 slots of the largest number, and what is far below that is off by less than 2^-100.
 // seen, held: a bit for each of the lane's slots, for the column and for the sequence; looked at where masked.
 template <int NB, int NP>
 __device__ __forceinline__ void values_by_codes(const uint8_t *at, int lane, bool masked, uint32_t seen, uint32_t held, float (&p)[8], Gathered<NB> &s)
@@ -790,8 +791,8 @@ __device__ __forceinline__ void values_by_codes(const uint8_t *at, int lane, boo
     const int n16 = lane & 15;
     ValuePart<NB> v;
     take_values<NB>(at, lane, v);
-    for (int i = 0; i < 8; ++i) p[i] *= 0x1p57f;   // 2^64 with the 2^7 they have: products with codes of 2^-133 stay normal numbers
     bf16x8 w[NP], middle[NP];
+    bool large = false;
     {
         float mid[8];
         for (int i = 0; i < 8; ++i) {
@@ -802,12 +803,26 @@ __device__ __forceinline__ void values_by_codes(const uint8_t *at, int lane, boo
         if (masked)
             for (int i = 0; i < 8; ++i)
                 if (!(held >> i & 1) || !(mid[i] == mid[i])) mid[i] = 0.0f;
+        for (int i = 0; i < 8; ++i) large = large || fabsf(mid[i]) >= 0x1p40f;
         split_bf16<NP>(mid, middle);
     }
-    split_bf16<NP>(p, w);
-    f32x4 low = zero;   // what block 4 g + r adds to all its values, times 2^64
+    const bool small = __builtin_amdgcn_ballot_w64(large) != 0;   // (p is to be)
+    if (small && !s.far) {
+        s.far = 1;
+        for (int i = 0; i < NB / 2; ++i)
+            for (int n = 0; n < 4; ++n)
+                for (int r = 0; r < 4; ++r) s.o[i][n][r] *= 0x1p-48f;
+    }
+    const float down = s.far ? 0x1p-48f : 1.0f, lift = small ? 0x1p-48f : 0x1p57f, back = small ? 1.0f : 0x1p-57f * down;
+    {
+        float lifted[8];
+        for (int i = 0; i < 8; ++i) lifted[i] = p[i] * lift;
+        split_bf16<NP>(lifted, w);
+    }
+    f32x4 low = zero;   // what block 4 g + r adds to all its values, times `lift` and the 2^7 of p
     for (int n = 0; n < NP; ++n)
         for (int e = 0; n + e < NP; ++e) low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(middle[n], w[e], low, 0, 0, 0);
+    for (int i = 0; i < 8; ++i) p[i] *= 0x1p57f;   // 2^64 with the 2^7 they have: products with codes of 2^-133 stay normal numbers
     for (int b = 0; b < NB; ++b) {
         float ps[8];
         for (int i = 0; i < 8; ++i) ps[i] = fmaf((float)v.steps[b][i], p[i], 0.0f);
@@ -817,7 +832,7 @@ __device__ __forceinline__ void values_by_codes(const uint8_t *at, int lane, boo
         }
         split_bf16<NP>(ps, w);
         const u32x4 codes = v.codes[b >> 1];
-        const float base = __shfl(low[b & 3], n16 + 16 * (b >> 2), 64) * 0x1p-57f;
+        const float base = __shfl(low[b & 3], n16 + 16 * (b >> 2), 64) * back;
         for (int n = 0; n < 2; ++n) {
             u32x4 c;
             for (int i = 0; i < 4; ++i) c[i] = code_pairs<kFineValues>(codes[i])[2 * (b & 1) + n];
@@ -827,7 +842,7 @@ __device__ __forceinline__ void values_by_codes(const uint8_t *at, int lane, boo
                 o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, c), w[e], o, 0, 0, 0);
                 o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{back, back, back, back}), w[e], o, 0, 0, 0);
             }
-            for (int r = 0; r < 4; ++r) s.o[b >> 1][2 * (b & 1) + n][r] += fmaf(o[r], kFineValues || n ? 0x1p72f : 0x1p76f, base);
+            for (int r = 0; r < 4; ++r) s.o[b >> 1][2 * (b & 1) + n][r] += fmaf(o[r], (kFineValues || n ? 0x1p72f : 0x1p76f) * down, base);
         }
     }
 }
@@ -898,7 +913,7 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
                 *(uint32_t *)(at + record_bytes(NB) + pair * 4) = __builtin_bit_cast(uint32_t, l);
             }
         }
-        numbers = __builtin_amdgcn_ballot_w64(!fine) == 0;
+        numbers = __builtin_amdgcn_ballot_w64(!fine) == 0 && !s.far;
         wave_lds_order();
     }
     float p[8], most = kNegInf;
@@ -948,6 +963,7 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
         x.sums = s;
         values_apart<NB>(at, lane, masked, seen, held, &x);
         s = x.sums;
+        s.far = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.far);
     }
 }
 
@@ -990,6 +1006,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
         for (int p = 0; p < 4; ++p) acc.o[i][p] = f32x4{0, 0, 0, 0};
     acc.top = kNegInf;
     acc.total = 0.0f;
+    acc.far = 0;
     uint8_t *stage = s_mem + wave * kStage;
     const f32x4 zero = kept_zero();
     const Under under = under_codes();
@@ -1014,9 +1031,10 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     float total = acc.total;
     const float top = acc.top;
 
-    // the waves' results meet in LDS
+    // the waves' results meet in LDS, as means: no sum of values is larger than they are
     total += __shfl_xor(total, 16, 64);
     total += __shfl_xor(total, 32, 64);
+    const float share = total == 0.0f ? 0.0f : 1.0f / total, raise = acc.far ? 0x1p48f : 1.0f;   // (both times 2^7)
     if (g == 0) {
         s_top[wave][n] = top;
         s_total[wave][n] = total * 0x1p-7f;
@@ -1024,7 +1042,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     for (int i = 0; i < NB / 2; ++i) {
         for (int p = 0; p < 4; ++p) {
             f32x4 v;
-            for (int r = 0; r < 4; ++r) v[r] = acc.o[i][p][r] * 0x1p-7f;
+            for (int r = 0; r < 4; ++r) v[r] = acc.o[i][p][r] * share * raise;
             *(f32x4 *)&s_o[wave][n][64 * i + 16 * p + 4 * g] = v;
         }
     }
@@ -1032,14 +1050,16 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
     const int column = threadIdx.x >> 4, part = threadIdx.x & 15;
     float all = kNegInf;
     for (int w = 0; w < kAttendWaves; ++w) all = fmaxf(all, s_top[w][column]);
-    float sum = 0.0f, x[2 * NB];
+    float sum = 0.0f, of[kAttendWaves], x[2 * NB];
     for (int i = 0; i < 2 * NB; ++i) x[i] = 0.0f;
     for (int w = 0; w < kAttendWaves; ++w) {
         // (a wave that saw nothing holds zeros; with a NaN among what it saw its total is one)
-        const float f = all == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(s_top[w][column] - all);
-        sum = fmaf(s_total[w][column], f, sum);
-        for (int i = 0; i < 2 * NB; ++i) x[i] = fmaf(s_o[w][column][part * 2 * NB + i], f, x[i]);
+        of[w] = s_total[w][column] * (all == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(s_top[w][column] - all));
+        sum += of[w];
     }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int w = 0; w < kAttendWaves; ++w)
+        for (int i = 0; i < 2 * NB; ++i) x[i] = fmaf(s_o[w][column][part * 2 * NB + i], of[w] * inv, x[i]);
     if (tile * kColumns + column >= count * a.group) return;
     if (a.splits > 1) {
         const uint64_t at = ((uint64_t)unit * kColumns + (uint32_t)column) * (uint32_t)a.splits + (uint32_t)split;
@@ -1358,7 +1378,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
         const int row = column / a.group, head = column - row * a.group;
         const uint64_t line = (uint64_t)(first + row) * a.out_row_stride + (uint64_t)(h * a.group + head) * a.out_head_stride;
         const uint64_t place = (((uint64_t)(unit / (unsigned)a.wide_tiles) * (unsigned)a.tiles + (unsigned)tile) * kColumns + (unsigned)n) * (unsigned)a.splits + (unsigned)split;
-        const float scale = a.splits > 1 ? 0x1p-7f : (total == 0.0f ? 0.0f : 0x1p-7f / total);
+        const float scale = total == 0.0f ? 0.0f : 0x1p-7f / total;
         for (int i = 0; i < NB / 2; ++i) {
             for (int p = 0; p < 4; ++p) {
                 float v[4];
@@ -1378,8 +1398,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
     }
 }
 
-// Joins the parts of a column: a workgroup each, its waves taking parts in turn, 2 NB of the column's values a lane (the waves' other
-// lanes further parts).
+// Joins the parts of a column, means and sums of weights: a workgroup each, its waves taking parts in turn, 2 NB of the column's values a lane (the
+// waves' other lanes further parts).
 template <int NB, int TY>
 __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
 {
@@ -1409,23 +1429,28 @@ __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
     if (place == 0) s_top[strand] = top;
     __syncthreads();
     for (int k = 0; k < kStrands; ++k) top = fmaxf(top, s_top[k]);
-    for (int k = strand; k < parts; k += kStrands) {
+    auto weight = [&](int k) __attribute__((always_inline)) {
         const uint64_t p = at + (uint32_t)k;
-        const float f = top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(a.partial_sums[2 * p] - top);
+        return a.partial_sums[2 * p + 1] * (top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(a.partial_sums[2 * p] - top));
+    };
+    float own = 0.0f;
+    for (int k = strand; k < parts; k += kStrands) own += weight(k);
+    if (place == 0) s_total[strand] = own;
+    __syncthreads();
+    for (int k = 0; k < kStrands; ++k) total += s_total[k];
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    for (int k = strand; k < parts; k += kStrands) {
         float y[2 * NB];
-        load_run<2 * NB>(a.partial, p * D + (uint32_t)(place * 2 * NB), y);
-        total = fmaf(a.partial_sums[2 * p + 1], f, total);
+        load_run<2 * NB>(a.partial, (at + (uint32_t)k) * D + (uint32_t)(place * 2 * NB), y);
+        const float f = weight(k) * inv;
         for (int i = 0; i < 2 * NB; ++i) x[i] = fmaf(y[i], f, x[i]);
     }
     for (int i = 0; i < 2 * NB; ++i) s_sum[strand][place * 2 * NB + i] = x[i];
-    if (place == 0) s_total[strand] = total;
     __syncthreads();
     if (strand != 0) return;
     const int strands = parts < kStrands ? parts : kStrands;
-    for (int k = 1; k < strands; ++k) {
-        total += s_total[k];
+    for (int k = 1; k < strands; ++k)
         for (int i = 0; i < 2 * NB; ++i) x[i] += s_sum[k][place * 2 * NB + i];
-    }
     write_result<NB, TY>(a, h, first, tile * kColumns + column, place, top, total, x);
 }
 
