@@ -1,4 +1,6 @@
 """Further checks of the 4-bit cache for both places to run it (cache_world.py): calls in which not all is as wide as it could be."""
+from fractions import Fraction
+
 import numpy as np
 import torch
 
@@ -89,3 +91,70 @@ def far_and_tiny_values(k, v, slots):
 
 
 FAR = [far_values, farthest_values, only_farthest_values, last_value_far, far_and_tiny_values]
+
+
+# ---------------------------------------------------------------- the codec's decisions in exact arithmetic
+POSITIVE = [Fraction(float(v)) for v in ref.bf16_values(np.arange(0x7f80))]                             # 0 and the positive bfloat16, ascending
+STEPS = [Fraction(float(v)) for v in np.arange(0x7c00, dtype=np.uint16).view(np.float16)]
+
+
+def exact_block(x):
+    """(codes, s, lo) of 32 finite numbers of 32 bits from the header's definition, in rational numbers."""
+    x = [Fraction(float(v)) for v in x]
+    low, high = min(x), max(x)
+    up, steps = POSITIVE, STEPS
+    if low >= 0:
+        a, b = 0, len(up) - 1                                  # the largest not above
+        while a < b:
+            m = (a + b + 1) // 2
+            a, b = (m, b) if up[m] <= low else (a, m - 1)
+        lo = up[a]
+    else:
+        a, b = 0, len(up) - 1                                  # of the negated ones the smallest not below
+        while a < b:
+            m = (a + b) // 2
+            a, b = (a, m) if up[m] >= -low else (m + 1, b)
+        lo = -up[a]
+    if 15 * steps[-1] < high - lo:
+        return [0] * 32, float("nan"), 0.0
+    a, b = 0, len(steps) - 1
+    while a < b:
+        m = (a + b) // 2
+        a, b = (a, m) if 15 * steps[m] >= high - lo else (m + 1, b)
+    s = steps[a]
+    codes = [0 if s == 0 else sum(v >= lo + (j + Fraction(1, 2)) * s for j in range(15)) for v in x]
+    return codes, float(s), float(lo)
+
+
+def hard_blocks(seed=0, n=40):
+    """Blocks whose borders take more than 64 bits: a lowest number far below the step, exact half steps, their neighbours."""
+    rng = np.random.default_rng(seed)
+    out = [[1e-30, 15, 0.5, 2.5] + [1] * 28, [-1e-30, 15, 0.5, 2.5, 14.5] + [1] * 27, [1e-30, 30, 1, 3, 5, 29] + [2] * 26,
+           [-1e-30, 30, 1, 3, 5, 29] + [2] * 26, [-0.5, 14.5, 1e-30, -1e-30, 0.0, -0.0, 1e-45, -1e-45] + [3] * 24,
+           [1e-45, 2.0 ** -24 * 15, 2.0 ** -25, 3 * 2.0 ** -25] + [0.0] * 28, [-1e-45, 2.0 ** -24 * 15, 2.0 ** -25, 3 * 2.0 ** -25] + [0.0] * 28,
+           [-1e-40] * 31 + [1e-40], [1e-40, 65504.0 * 15] + [32752.0] * 30, [-1e-40, 65504.0 * 15] + [1.0] * 30]
+    for _ in range(n):
+        s = float(np.float16(2.0 ** rng.integers(-20, 12) * rng.integers(1024, 2048) / 1024))
+        lo = float(torch.tensor(rng.choice([-1, 1]) * 2.0 ** float(rng.integers(-120, 12))).bfloat16())
+        at = lo + (rng.integers(0, 15, 32) + rng.choice([0.0, 0.5], 32)) * s
+        x = at.astype(np.float32)
+        x = np.where(rng.random(32) < 0.3, np.nextafter(x, np.float32(np.inf)), np.where(rng.random(32) < 0.3, np.nextafter(x, np.float32(-np.inf)), x))
+        x[0], x[1] = lo, np.float32(lo + 15 * s)
+        out.append(np.maximum(x, np.float32(lo)).tolist())
+    return np.array(out, np.float32)
+
+
+def check_store_exact(world, blocks):
+    """Codes, steps and lowest numbers bit for bit what rational arithmetic says, keys and values."""
+    n = len(blocks) // 2
+    b = Batch(world, [n], [n], 1, 64, 32)
+    x = world.put(np.ascontiguousarray(blocks[:2 * n].reshape(n, 1, 64)))
+    b.c.store(x, x, b.d_table, b.d_lengths, b.d_starts)
+    raw = b.raw()
+    for r in range(n):
+        key, value, _ = raw.row(int(b.table[0, r // 32]), 0, r % 32)
+        for i in range(2):
+            codes, s, lo = exact_block(blocks[2 * r + i])
+            for got, what in ((key, "key"), (value, "value")):
+                assert np.array_equal([got[1][i], got[2][i]], [s, lo], equal_nan=True), (what, blocks[2 * r + i], got[1][i], s, got[2][i], lo)
+                assert got[0][32 * i:32 * i + 32].tolist() == codes, (what, blocks[2 * r + i])

@@ -1,7 +1,7 @@
 """Further cases of the 4-bit cache on the CPU execution model."""
 import pytest
 
-from cache_cases import FAR, check_rows_left_out
+from cache_cases import FAR, check_rows_left_out, check_store_exact, hard_blocks
 from cache_world import check_attend
 from test_emu_cache import _release, world  # noqa: F401
 
@@ -25,3 +25,8 @@ def test_rows_left_out(world, rows, max_rows, hold, causal, window, group, type_
 ])
 def test_attend_far_values(world, edit, lengths, rows, group, d, type_, kw):  # noqa: F811
     check_attend(world, lengths, rows, 1, group, d, 32, type_, edit=edit, **kw)
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+def test_store_decides_exactly(world, seed):  # noqa: F811
+    check_store_exact(world, hard_blocks(seed, 40))

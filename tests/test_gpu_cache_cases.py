@@ -1,7 +1,7 @@
 """Further cases of the 4-bit cache on the GPU."""
 import pytest
 
-from cache_cases import FAR, check_rows_left_out
+from cache_cases import FAR, check_rows_left_out, check_store_exact, hard_blocks
 from cache_world import check_attend
 from test_emu_cache_cases import LEFT_OUT
 from test_gpu_cache import world  # noqa: F401
@@ -24,3 +24,8 @@ def test_rows_left_out(world, rows, max_rows, hold, causal, window, group, d, ty
 ])
 def test_attend_far_values(world, edit, lengths, rows, group, d, type_, kw):  # noqa: F811
     check_attend(world, lengths, rows, 1, group, d, 32, type_, edit=edit, **kw)
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+def test_store_decides_exactly(world, seed):  # noqa: F811
+    check_store_exact(world, hard_blocks(seed, 400))

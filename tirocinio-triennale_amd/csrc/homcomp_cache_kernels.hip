@@ -181,10 +181,19 @@ __device__ __forceinline__ uint32_t of_quad(uint32_t x)
 template <int XOR>
 __device__ __forceinline__ float of_quad(float x) { return __builtin_bit_cast(float, of_quad<XOR>(__builtin_bit_cast(uint32_t, x))); }
 
-// Eight values a lane.  All decisions are those of exact arithmetic: the borders lo + (j + 1/2) s have at most 44 significant bits (s is at
-// least a fifteenth of the range, lo at most 2^8 of its own last places), so 64-bit floats hold them.  In 32 bits (x - lo) / s + 1/2 is
-// at most 15 1/2 and off by the roundings of the difference and the sum and the reciprocal's 2^-23: under 64 * 2^-24 = 2^-18.
-// Only where a value is within 2^-17 of a border, in about one wave of a hundred, are the borders looked at.
+// What a + b, rounded to `sum`, lost: a number of its own (the two-sum of Knuth).
+__device__ __forceinline__ double lost(double a, double b, double sum)
+{
+    const double of_b = sum - a, of_a = sum - of_b;
+    return (a - of_a) + (b - of_b);
+}
+
+// Eight values a lane.  All decisions are those of exact arithmetic: the range and the borders lo + (j + 1/2) s have at most 44 significant bits (s is at
+// least a fifteenth of the range, lo at most 2^8 of its own last places), so 64-bit floats hold them, unless lo and the largest value are far
+// apart (1e-30 beside 15).  There a rounded sum still compares rightly with another number, but for a tie: what it lost decides.  In 32 bits
+// (x - lo) / s + 1/2 is at most 15 1/2 and off by the roundings of the difference and the sum and the reciprocal's 2^-23: under
+// 64 * 2^-24 = 2^-18.  Only where a value is within 2^-17 of a border are the borders looked at: in one wave of a hundred, and in
+// one of five where values are bfloat16, whose differences from lo hit some borders exactly.
 __device__ __forceinline__ Block8 quantise(const float *x)
 {
     float mn = x[0], mx = x[0], odd = 0.0f;
@@ -226,6 +235,37 @@ __device__ __forceinline__ Block8 quantise(const float *x)
             const double v = (double)x[i], at = (double)c;
             if (c < 15 && v >= fma(at + 0.5, (double)s, (double)lo)) r.code[i] = c + 1;
             else if (c > 0 && v < fma(at - 0.5, (double)s, (double)lo)) r.code[i] = c - 1;
+        }
+    }
+    const float lesser = fminf(fabsf(mx), fabsf(lo));
+    if (lesser < fmaxf(fabsf(mx), fabsf(lo)) * 0x1p-20f && lesser > 0.0f && !none) {
+        // far apart (seldom): a step that only seemed to reach, then every code anew, from an estimate that is at most one off.  (A loop whose
+        // body takes the first of the values and turns them round: in line it is much code for every block.)
+        if (15.0 * (double)s == range && lost((double)mx, -(double)lo, range) > 0.0) ++r.s;
+        const double step = (double)f16_to_f32(r.s);
+        const float rstep = __builtin_amdgcn_rcpf((float)step);
+        float y[8];
+        for (int i = 0; i < 8; ++i) y[i] = x[i];
+#pragma unroll 1
+        for (int n = 0; n < 8; ++n) {
+            uint32_t c = (uint32_t)fmaxf(fmaf(y[0] - lo, rstep, 0.5f), 0.5f);
+            auto reaches = [&](double halves) __attribute__((always_inline)) {   // the border lo + halves s
+                const double v = (double)y[0], border = (double)lo + halves * step;
+                return v > border || (v == border && lost((double)lo, halves * step, border) <= 0.0);
+            };
+            if (c < 15 && reaches((double)c + 0.5)) ++c;
+            else if (c > 0 && !reaches((double)c - 0.5)) --c;
+            const float first = y[0];
+            for (int i = 0; i < 7; ++i) {
+                y[i] = y[i + 1];
+                r.code[i] = r.code[i + 1];
+            }
+            y[7] = first;
+            r.code[7] = r.s < 0x7c00u ? c : 0;
+        }
+        if (r.s >= 0x7c00u) {   // (the step was the largest one)
+            r.s = 0x7e00u;
+            r.lo = 0;
         }
     }
     return r;
