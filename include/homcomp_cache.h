@@ -41,6 +41,7 @@
  *     sequence's last slot is never part of a result.
  *   - Two calls that touch the same slots or the same scratch memory have to be ordered by the caller (one stream, or events).
  *     Sequences may have pages in common; rows that one call writes must have slots of their own.
+ *   - Rows of numbers that a call writes (of out, or of the arrays that a load fills) share no memory, with one another or with what it reads.
  *   - A call of more workgroups than a launch can have (2^24 - 1 of 256 threads) is refused.
  */
 #ifndef HOMCOMP_CACHE_H

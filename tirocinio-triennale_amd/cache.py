@@ -87,6 +87,33 @@ def _allocating(stream):
 _NOTHING = contextlib.nullcontext()
 
 
+def _share_memory(rows, row, heads, head, d):
+    """Whether of the runs of d elements at i * row + j * head two have one in common."""
+    if rows > 1 and row < d or heads > 1 and head < d:
+        return True
+    if rows < 2 or heads < 2 or row >= (heads - 1) * head + d or head >= (rows - 1) * row + d:
+        return False                      # (one inside the other: nearly every layout)
+    for j in range(1, heads):             # j heads on and the rows next to there
+        i = j * head // row
+        if i < rows and j * head - i * row < d or i + 1 < rows and (i + 1) * row - j * head < d:
+            return True
+    return False
+
+
+def _meet(offset, rows, row, heads, head, d):
+    """Whether the runs of two such arrays, the second `offset` elements behind the first, have an element in common."""
+    offset = abs(offset)
+    row, head = row if rows > 1 else 0, head if heads > 1 else 0
+    if offset >= (rows - 1) * row + (heads - 1) * head + d:
+        return False
+    for j in range(1 - heads, heads):     # offset + j * head against the rows next to there, of either sign
+        at = offset + j * head
+        i = at // row if row else 0
+        if min(abs(at - max(1 - rows, min(rows - 1, x)) * row) for x in (i, i + 1)) < d:
+            return True
+    return False
+
+
 class Cache:
     """Pages of a cache and their shape.  The tables and lengths that say whose slots they are belong to the calls:
 
@@ -154,7 +181,7 @@ class Cache:
 
     def _own_memory(self, name, t, row, head):
         """Written tensors: no row or head of which shares another's memory."""
-        if t.numel() and (row == 0 and t.shape[0] > 1 or head == 0 and t.shape[1] > 1):
+        if t.numel() and _share_memory(t.shape[0], row, t.shape[1], head, self.head_dim):
             raise ValueError(f"{name}: rows and heads of its own memory")
 
     def _whole(self, name, t, shape, dtype):
@@ -168,6 +195,8 @@ class Cache:
             raise ValueError("k and v: of one type, shape and layout")
         if written:
             self._own_memory("k and v", k, row, head)
+            if k.numel() and _meet((v.data_ptr() - k.data_ptr()) // k.element_size(), k.shape[0], row, k.shape[1], head, self.head_dim):
+                raise ValueError("k and v: each of its own memory")
         args, n, _ = self._args(table, lengths)
         self._call(name, what, args, k.data_ptr(), v.data_ptr(), self._types[k.dtype], row, head, self._starts(starts, n), k.shape[0],
                    _stream_of(self._device, stream))
