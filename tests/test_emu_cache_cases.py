@@ -1,7 +1,7 @@
 """Further cases of the 4-bit cache on the CPU execution model."""
 import pytest
 
-from cache_cases import FAR, check_rows_left_out, check_store_exact, hard_blocks
+from cache_cases import FAR, check_rows_left_out, check_store_exact, close_keys, close_queries, hard_blocks
 from cache_world import check_attend
 from test_emu_cache import _release, world  # noqa: F401
 
@@ -30,3 +30,10 @@ def test_attend_far_values(world, edit, lengths, rows, group, d, type_, kw):  # 
 @pytest.mark.parametrize("seed", [0, 1])
 def test_store_decides_exactly(world, seed):  # noqa: F811
     check_store_exact(world, hard_blocks(seed, 40))
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.5, 4.0])
+@pytest.mark.parametrize("rows,group", [(1, 2), (10, 3)])
+def test_large_scores_close_together(world, rows, group, scale, type_):  # noqa: F811
+    check_attend(world, [250], [rows], 1, group, 64, 32, type_, scale=scale, edit=close_keys, q_edit=close_queries)

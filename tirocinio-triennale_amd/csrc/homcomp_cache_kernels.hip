@@ -1211,8 +1211,9 @@ __device__ __forceinline__ bool lay_unit(uint8_t *at, const uint8_t *sides, cons
 }
 template <int NB>
 struct WideGathered {
-    f32x4 o[NB / 2][4];   // sum of value * p, values 64 i + 16 p + 4 g + r, times 2^7
-    float top, total;     // as in Gathered; total times 2^7
+    f32x4 o[NB / 2][4];   // sum of value * p, values 64 i + 16 p + 4 g + r
+    float top;            // exponent p is relative to, one that 32 bits hold: about 7 below the largest so far, at most 15
+    float total;          // sum of the lane's p
 };
 
 // The CT tiles of a wave together: what is read from LDS serves all of them.
@@ -1248,7 +1249,8 @@ __device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB,
         }
         float most = kNegInf;
         for (int i = 0; i < 8; ++i) most = fmaxf(most, e[t][i >> 2][i & 3]);
-        higher = higher || most > s[t].top + 8.0f;
+        // (p up to 2^15: float16 has room for that.  The difference, not a sum with top: numbers of 2^25 and more are whole fours and further apart)
+        higher = higher || most - s[t].top > 15.0f;
     }
     if (__builtin_amdgcn_ballot_w64(higher) != 0) {
         for (int t = 0; t < CT; ++t) {
@@ -1256,7 +1258,7 @@ __device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB,
             for (int i = 0; i < 8; ++i) most = fmaxf(most, e[t][i >> 2][i & 3]);
             most = fmaxf(most, __shfl_xor(most, 16, 64));
             most = fmaxf(most, __shfl_xor(most, 32, 64));
-            const float now = fmaxf(s[t].top, most);
+            const float now = fmaxf(s[t].top, most - 7.0f);
             const float shrink = now == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(s[t].top - now);
             s[t].top = now;
             s[t].total *= shrink;
@@ -1267,9 +1269,9 @@ __device__ __forceinline__ void attend_wide(const uint8_t *at, const Queries<NB,
     }
     f16x8 w[CT][NP];
     for (int t = 0; t < CT; ++t) {
-        const float bias = s[t].top == kNegInf ? 7.0f : 7.0f - s[t].top;
+        const float top = s[t].top == kNegInf ? 0.0f : s[t].top;
         for (int i = 0; i < 8; ++i) {
-            const float p = __builtin_amdgcn_exp2f(e[t][i >> 2][i & 3] + bias);
+            const float p = __builtin_amdgcn_exp2f(e[t][i >> 2][i & 3] - top);
             s[t].total += p;
             w[t][0][i] = (_Float16)p;
             if (NP == 2) w[t][NP - 1][i] = (_Float16)(p - (float)w[t][0][i]);
@@ -1413,12 +1415,11 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
         float total = acc[t].total;
         total += __shfl_xor(total, 16, 64);
         total += __shfl_xor(total, 32, 64);
-        total *= 0x1p-7f;
         if (column >= count * a.group) continue;
         const int row = column / a.group, head = column - row * a.group;
         const uint64_t line = (uint64_t)(first + row) * a.out_row_stride + (uint64_t)(h * a.group + head) * a.out_head_stride;
         const uint64_t place = (((uint64_t)(unit / (unsigned)a.wide_tiles) * (unsigned)a.tiles + (unsigned)tile) * kColumns + (unsigned)n) * (unsigned)a.splits + (unsigned)split;
-        const float scale = total == 0.0f ? 0.0f : 0x1p-7f / total;
+        const float scale = total == 0.0f ? 0.0f : 1.0f / total;
         for (int i = 0; i < NB / 2; ++i) {
             for (int p = 0; p < 4; ++p) {
                 float v[4];
