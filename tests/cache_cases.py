@@ -173,3 +173,20 @@ def close_queries(q):
     q[:] = 0.0
     q[:, :, 0] = 8192.0
     q[:, :, 32] = 2.77
+
+
+# ---------------------------------------------------------------- queries and scales near the end of 32 bits, scores inside it
+def small_constant_keys(k, v, slots):
+    k[:] = (2.0 ** -100 * (1 + slots % 7 / 8.0))[:, None, None]
+
+
+def largest_queries(q):
+    """Columns of 2^121 and more beside ordinary ones and small ones."""
+    q[:, 0] *= 2.0 ** 122
+    q[:, 1:2] *= 2.0 ** 60
+    q[-1, -1] *= 2.0 ** -20
+
+
+FAR_QUERIES = [
+    dict(q_scale=1e37), dict(q_scale=1e37, scale=1e-3), dict(q_scale=1e5, scale=1e31), dict(q_scale=3.0, scale=-1e36), dict(q_scale=1e37, scale=1e-37),
+    dict(q_edit=largest_queries, edit=small_constant_keys), dict(q_edit=largest_queries, scale=0.01), dict(q_scale=1e-30, scale=1e37)]

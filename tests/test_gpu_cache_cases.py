@@ -1,7 +1,7 @@
 """Further cases of the 4-bit cache on the GPU."""
 import pytest
 
-from cache_cases import FAR, check_rows_left_out, check_store_exact, close_keys, close_queries, hard_blocks
+from cache_cases import FAR, FAR_QUERIES, check_rows_left_out, check_store_exact, close_keys, close_queries, hard_blocks
 from cache_world import check_attend
 from test_emu_cache_cases import LEFT_OUT
 from test_gpu_cache import world  # noqa: F401
@@ -36,3 +36,10 @@ def test_store_decides_exactly(world, seed):  # noqa: F811
 @pytest.mark.parametrize("rows,group", [(1, 2), (10, 3)])
 def test_large_scores_close_together(world, rows, group, scale, type_):  # noqa: F811
     check_attend(world, [250], [rows], 1, group, 64, 32, type_, scale=scale, edit=close_keys, q_edit=close_queries)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f32"])   # (float16 queries do not reach that far)
+@pytest.mark.parametrize("kw", FAR_QUERIES)
+@pytest.mark.parametrize("lengths,rows,group", [([40], [1], 2), ([100], [9], 3), ([300], [2], 3)])
+def test_largest_queries_and_scales(world, lengths, rows, group, kw, type_):  # noqa: F811
+    check_attend(world, lengths, rows, 1, group, 64, 32, type_, **kw)

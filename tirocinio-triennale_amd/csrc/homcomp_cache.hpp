@@ -47,7 +47,8 @@ struct AttendArgs {
     int32_t split_records;      // records of a part, a multiple of kAttendWaves
     int32_t q_aligned;          // every eight numbers of q lie at a multiple of 16 bytes
     int32_t causal, window;     // window 0: none
-    float scale;
+    float scale;                // of the scores, times log2 e: scale 2^scale_exponent
+    int32_t scale_exponent;
     float *lse;                 // null: not wanted
     float *partial;             // of more than one split: [tile][kColumns][split][head_dim], means
     float *partial_sums;        // [tile][kColumns][split][2]: exponent the part is relative to, sum

@@ -212,7 +212,7 @@ int homcomp_cache_attend(const homcomp_cache *cache, const homcomp_attention *t,
     a.q_aligned = eights_aligned(t->d_q, t->type, t->q_row_stride, t->q_head_stride) ? 1 : 0;
     a.causal = t->causal ? 1 : 0;
     a.window = t->window > (size_t)kMostSlots ? 0 : (int32_t)t->window;   // (no slot is that far away)
-    a.scale = t->scale;
+    a.scale = std::frexp(t->scale, &a.scale_exponent) * 1.4426950408889634f;
     a.lse = p.lse_bytes ? (float *)((uint8_t *)t->d_scratch + p.partial_bytes + p.sums_bytes) : t->d_lse;
     a.partial = (float *)t->d_scratch;
     a.partial_sums = (float *)((uint8_t *)t->d_scratch + p.partial_bytes);

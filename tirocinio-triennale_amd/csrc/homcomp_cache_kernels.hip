@@ -520,7 +520,8 @@ template <int NB, int NQ>
 struct Queries {
     f16x8 q[NB][NQ];    // values 32 b + 8 g .. + 7 of the column's row, scaled; where codes stand sixteen times as high by 1/16 more
     bf16x8 sums;        // g-th part (of three) of the sums over each block, times what the codes are
-    float factor;       // what turns a score into the exponent of a power of two
+    float factor;       // what turns a score into the exponent of a power of two, short of
+    int shift;          // 2^shift: 0 but for queries and scales near the end of 32 bits (the same in all lanes)
     int see_from, see_to;   // slots see_from <= j < see_to are seen
 };
 
@@ -603,7 +604,17 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
     split_bf16<3>(sums, parts);
     const bf16x8 none = __builtin_bit_cast(bf16x8, u32x4{0, 0, 0, 0});
     r.sums = g == 0 ? parts[0] : (g == 1 ? parts[1] : (g == 2 ? parts[2] : none));
-    r.factor = ldexpf(a.scale * kLog2e, (FORM == kWhole ? -14 : 10) + e);
+    int above = a.scale_exponent + (FORM == kWhole ? -14 : 10) + e - 126;
+    r.shift = 0;
+    if (__builtin_amdgcn_ballot_w64(above > 0) != 0) {
+        int most = above;
+        for (int lane = 1; lane < 16; lane *= 2) {
+            const int other = __shfl_xor(most, lane, 64);
+            most = other > most ? other : most;
+        }
+        r.shift = __builtin_amdgcn_readfirstlane(most);
+    }
+    r.factor = ldexpf(a.scale, above + 126 - r.shift);
     const int own = slot0 + row;
     r.see_to = !there ? 0 : (a.causal ? (own + 1 < length ? own + 1 : length) : length);
     r.see_from = a.window > 0 && own + 1 > a.window ? own + 1 - a.window : 0;
@@ -971,11 +982,12 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
         }
     }
     for (int i = 0; i < 8; ++i) most = fmaxf(most, p[i]);
-    if (__builtin_amdgcn_ballot_w64(most > 15.0f || !(fabsf(bias) < 0x1p16f)) != 0) {
+    if (__builtin_amdgcn_ballot_w64(most > 15.0f || !(fabsf(bias) < 0x1p16f)) != 0 || q.shift != 0) {
         float e[8];   // (rounded before the reference is taken off: with exponents above 2^16 the product's rounding would count)
         most = kNegInf;
         for (int i = 0; i < 8; ++i) {
             e[i] = x[i >> 2][i & 3] * q.factor;
+            if (q.shift != 0) e[i] = ldexpf(e[i], q.shift);
             if (seen >> i & 1) most = fmaxf(most, e[i]);
         }
         most = fmaxf(most, __shfl_xor(most, 16, 64));
@@ -1360,7 +1372,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_cache_attend_rows(AttendArgs 
             if (u < 2 * kPer * NB && rec) raw[k] = load_unit<NB>(rec, (u + r * NB) % (2 * NB), lane);
         }
     };
-    bool fine = true;
+    bool fine = true;   // (queries that need a shift are left to the other kernel too)
+    for (int t = 0; t < CT; ++t) fine = fine && q[t].shift == 0;
     const Under under = under_codes();
     auto lay_codes = [&](int j, const Pair &p) __attribute__((always_inline)) {
         for (int k = 0; k < kUnits; ++k) {
@@ -1578,7 +1591,7 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
     load_batch(begin);
     int tile = -1;
     Queries<NB, NQ> q;
-    float lse = 0.0f;
+    float less = 0.0f, up = 1.0f;   // the column's lse as an exponent, negative, short of up = 2^shift
     for (int it0 = begin; it0 < begin + kBatch * batches && it0 < held; it0 += kBatch) {
         // the columns of the next tile that sees any of the records (a single tile stays)
         int next = -1;
@@ -1592,11 +1605,13 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
             tile = next;
             const int column = tile * kColumns + n;
             load_queries<NB, TY, kFine>(a, h, first, count, slot0, length, column, g, q);
-            lse = 0.0f;
+            less = 0.0f;
             if (column < count * a.group) {
                 const int row = column / a.group, head = column - row * a.group;
-                lse = a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)];
+                less = a.lse[(uint64_t)(first + row) * ((uint64_t)a.c.kv_heads * a.group) + (uint64_t)(h * a.group + head)] * -kLog2e;
             }
+            less = ldexpf(less, -q.shift);
+            up = ldexpf(1.0f, q.shift);
             return true;
         };
         bool more = next_tile();
@@ -1619,7 +1634,7 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
                 const int from_slot = (it0 + k) * kRecordSlots + 8 * g;
                 for (int i = 0; i < 8; ++i)
                     if (sees(q, from_slot + i))
-                        sum[k][i] += __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, lse * -kLog2e));
+                        sum[k][i] += __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, less) * up);
             }
         }
         for (int k = 0; k < kHeldRecords; ++k) {
