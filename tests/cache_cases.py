@@ -190,3 +190,18 @@ def largest_queries(q):
 FAR_QUERIES = [
     dict(q_scale=1e37), dict(q_scale=1e37, scale=1e-3), dict(q_scale=1e5, scale=1e31), dict(q_scale=3.0, scale=-1e36), dict(q_scale=1e37, scale=1e-37),
     dict(q_edit=largest_queries, edit=small_constant_keys), dict(q_edit=largest_queries, scale=0.01), dict(q_scale=1e-30, scale=1e37)]
+
+
+def check_weights_of_large_scores(world, rows, group, type_, q_scale):
+    """Scores far above 2^16, where lse in 32 bits no longer says which share a slot has: a weight is still between 0 and the number of rows and
+    heads that count, and what lies outside what they see gets none."""
+    b = Batch(world, [90], [rows], 1, 64, 32, seed=2)
+    b.fill()
+    q = world.put((b.rng.standard_normal((rows, group, 64)) * q_scale).astype(np.float32), TYPES[type_])
+    out, weights = world.full((rows, group, 64), 0.0, TYPES[type_]), world.full((1, 1, 96), 33.0, torch.float32)
+    need = b.c.scratch_bytes(rows, group, 1, 3, TYPES[type_], weights=True)
+    b.c.attend(q, out, b.d_table, b.d_lengths, b.d_starts, weights=weights, scratch=world.full((need // 4 + 4,), float("nan"), torch.float32))
+    w = world.get(weights)[0, 0]
+    assert (w[:90] >= 0).all() and (w[:90] <= rows * group * (1 + rows * group * 2.0 ** -24)).all() and (w[90:] == 33.0).all(), w
+    assert (w[90 - np.arange(rows)[::-1] - 1] <= (np.arange(rows, 0, -1)) * group * (1 + 2.0 ** -20)).all()
+    assert np.isfinite(world.get(out)).all()

@@ -1,7 +1,7 @@
 """Further cases of the 4-bit cache on the CPU execution model."""
 import pytest
 
-from cache_cases import FAR, FAR_QUERIES, check_rows_left_out, check_store_exact, close_keys, close_queries, hard_blocks
+from cache_cases import FAR, FAR_QUERIES, check_rows_left_out, check_store_exact, check_weights_of_large_scores, close_keys, close_queries, hard_blocks
 from cache_world import check_attend
 from test_emu_cache import _release, world  # noqa: F401
 
@@ -44,3 +44,10 @@ def test_large_scores_close_together(world, rows, group, scale, type_):  # noqa:
 @pytest.mark.parametrize("lengths,rows,group", [([40], [1], 2), ([100], [9], 3), ([300], [2], 3)])
 def test_largest_queries_and_scales(world, lengths, rows, group, kw, type_):  # noqa: F811
     check_attend(world, lengths, rows, 1, group, 64, 32, type_, **kw)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f32"])
+@pytest.mark.parametrize("q_scale", [1e6, 1e9, 1e20, 1e36])
+@pytest.mark.parametrize("rows,group", [(1, 3), (7, 4)])
+def test_weights_of_large_scores(world, rows, group, q_scale, type_):  # noqa: F811
+    check_weights_of_large_scores(world, rows, group, type_, q_scale)

@@ -1591,7 +1591,8 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
     load_batch(begin);
     int tile = -1;
     Queries<NB, NQ> q;
-    float less = 0.0f, up = 1.0f;   // the column's lse as an exponent, negative, short of up = 2^shift
+    // the column's lse as an exponent, negative, short of up = 2^shift; one: a NaN where lse is one
+    float less = 0.0f, up = 1.0f, one = 1.0f;
     for (int it0 = begin; it0 < begin + kBatch * batches && it0 < held; it0 += kBatch) {
         // the columns of the next tile that sees any of the records (a single tile stays)
         int next = -1;
@@ -1612,6 +1613,7 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
             }
             less = ldexpf(less, -q.shift);
             up = ldexpf(1.0f, q.shift);
+            one = fmaf(less, 0.0f, 1.0f);
             return true;
         };
         bool more = next_tile();
@@ -1632,9 +1634,11 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
                 f32x4 x[2];
                 record_scores<NB, NQ, true>(keys, q, f32x4{0, 0, 0, 0}, x);
                 const int from_slot = (it0 + k) * kRecordSlots + 8 * g;
-                for (int i = 0; i < 8; ++i)
-                    if (sees(q, from_slot + i))
-                        sum[k][i] += __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, less) * up);
+                for (int i = 0; i < 8; ++i) {
+                    // (between 0 and 1: an output modifier of the power's instruction, which makes a NaN a 0)
+                    const float w = fminf(fmaxf(__builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3], q.factor, less) * up), 0.0f), 1.0f);
+                    if (sees(q, from_slot + i)) sum[k][i] = fmaf(w, one, sum[k][i]);
+                }
             }
         }
         for (int k = 0; k < kHeldRecords; ++k) {
