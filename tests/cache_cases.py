@@ -205,3 +205,19 @@ def check_weights_of_large_scores(world, rows, group, type_, q_scale):
     assert (w[:90] >= 0).all() and (w[:90] <= rows * group * (1 + rows * group * 2.0 ** -24)).all() and (w[90:] == 33.0).all(), w
     assert (w[90 - np.arange(rows)[::-1] - 1] <= (np.arange(rows, 0, -1)) * group * (1 + 2.0 ** -20)).all()
     assert np.isfinite(world.get(out)).all()
+
+
+def check_lse_without_and_with_weights(world, type_, d, lengths=(300, 40)):
+    """The same scores whether or not weights are asked for: out and lse bit for bit."""
+    b = Batch(world, lengths, [2] * len(lengths), 2, d, 32, seed=3)
+    b.fill()
+    q = world.put(b.rng.standard_normal((b.total, 6, d)).astype(np.float32), TYPES[type_])
+    results = []
+    for weights in (False, True):
+        out, lse = world.full((b.total, 6, d), 0.0, TYPES[type_]), world.full((b.total, 6), 0.0, torch.float32)
+        width = b.table.shape[1] * 32
+        need = b.c.scratch_bytes(b.total, 6, len(lengths), b.table.shape[1], TYPES[type_], weights=weights, lse=True, max_rows=2)
+        kw = dict(weights=world.full((len(lengths), 2, width), 0.0, torch.float32)) if weights else {}
+        b.c.attend(q, out, b.d_table, b.d_lengths, b.d_starts, lse=lse, max_rows=2, scratch=world.full((need // 4 + 4,), float("nan"), torch.float32), **kw)
+        results.append((world.get(out), world.get(lse)))
+    assert np.array_equal(results[0][0], results[1][0]) and np.array_equal(results[0][1], results[1][1])

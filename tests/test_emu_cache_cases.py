@@ -1,7 +1,8 @@
 """Further cases of the 4-bit cache on the CPU execution model."""
 import pytest
 
-from cache_cases import FAR, FAR_QUERIES, check_rows_left_out, check_store_exact, check_weights_of_large_scores, close_keys, close_queries, hard_blocks
+from cache_cases import (FAR, FAR_QUERIES, check_lse_without_and_with_weights, check_rows_left_out, check_store_exact, check_weights_of_large_scores,
+                         close_keys, close_queries, hard_blocks)
 from cache_world import check_attend
 from test_emu_cache import _release, world  # noqa: F401
 
@@ -51,3 +52,9 @@ def test_largest_queries_and_scales(world, lengths, rows, group, kw, type_):  # 
 @pytest.mark.parametrize("rows,group", [(1, 3), (7, 4)])
 def test_weights_of_large_scores(world, rows, group, q_scale, type_):  # noqa: F811
     check_weights_of_large_scores(world, rows, group, type_, q_scale)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [64, 256])
+def test_lse_without_and_with_weights(world, d, type_):  # noqa: F811
+    check_lse_without_and_with_weights(world, type_, d)

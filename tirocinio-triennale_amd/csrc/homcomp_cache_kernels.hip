@@ -494,7 +494,7 @@ __global__ __launch_bounds__(256) void k_cache_load(CacheArgs c, RowsArgs a, uin
 //
 // Codes enter the matrix instructions as they are stored.  A nibble in the low bits of a 16-bit lane is a float16 or bfloat16 below
 // the normal range: the float16 of bits c is c 2^-24 and that of 16 c is c 2^-20, the bfloat16 are c 2^-133 and c 2^-129, exactly, and the
-// matrix unit takes them at their value.  So an AND (and one shift for every two) is all a pair of codes costs.
+// matrix unit takes them at their value.  So an AND and at most one shift is all a pair of codes costs.
 //   scores   S[slot, column] = sum_b s_b[slot] (sum_{j in b} c_j q_j) + sum_b lo_b[slot] (sum_{j in b} q_j)
 //            one 16x16x32 product per block of 32 values with slots as rows; its result is scaled in 32 bits.  q is float16, scaled by a power
 //            of two of its own row so that its largest value is near 2^14 (nothing that counts falls below float16's range), in three
@@ -518,7 +518,7 @@ constexpr int query_parts() { return TY == kF32 ? 3 : 1; }
 
 template <int NB, int NQ>
 struct Queries {
-    f16x8 q[NB][NQ];    // values 32 b + 8 g .. + 7 of the column's row, scaled; where codes stand sixteen times as high by 1/16 more
+    f16x8 q[NB][NQ];    // values 32 b + 8 g .. + 7 of the column's row, scaled; with codes at bits 4 .. 7 (sixteen times as high) by 1/16 more
     bf16x8 sums;        // g-th part (of three) of the sums over each block, times what the codes are
     float factor;       // what turns a score into the exponent of a power of two, short of
     int shift;          // 2^shift: 0 but for queries and scales near the end of 32 bits (the same in all lanes)
@@ -550,8 +550,8 @@ __device__ __forceinline__ void split_bf16(const float *x, bf16x8 *out)
 }
 
 // column: row * group + head of the group, at or beyond `columns` none (it sees no slot).
-// How codes enter the products of the scores: see code_pairs; kWhole: as the numbers c themselves.
-enum : int { kLow = 0, kFine = 1, kWhole = 2 };
+// How codes enter the products of the scores.  kFine: see code_pairs; kWhole: keys as numbers, lo + s c.
+enum : int { kFine = 0, kWhole = 1 };
 template <int NB, int TY, int FORM>
 __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int first, int count, int slot0, int length, int column, int g,
                                              Queries<NB, query_parts<TY>()> &r)
@@ -596,7 +596,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs &a, int h, int fir
             for (int i = 0; i < 8; ++i) {
                 const _Float16 part = (_Float16)rest[i];
                 rest[i] -= (float)part;
-                r.q[b][p][i] = FORM == kFine || (FORM == kLow && (i & 2)) ? (_Float16)((float)part * 0.0625f) : part;
+                r.q[b][p][i] = FORM == kFine ? (_Float16)((float)part * 0.0625f) : part;
             }
         }
     }
@@ -704,7 +704,8 @@ __device__ __forceinline__ void take_values(const uint8_t *at, int lane, ValuePa
 // The four pairs of codes of a word, as numbers of 16 bits below or at the foot of the normal range.  FINE: all at bits 4 .. 7, for two
 // more shifts: the matrix unit aligns products by their exponents, a number below the normal range counts as if it
 // had the smallest one, and what a product has in front of its first bit it lacks behind the last (measured for a score of a few
-// units: 4e-6 off with codes at bits 0 .. 3, 3e-7 at bits 4 .. 7).
+// units: 4e-6 off with codes at bits 0 .. 3, 3e-7 at bits 4 .. 7).  So scores, which lse and the weights are made of, take that form, whatever the type
+// of the results: 0.5 us of 91 for a batch of 64 sequences.  Values for 16-bit results take the other.
 template <bool FINE>
 __device__ __forceinline__ u32x4 code_pairs(uint32_t w)
 {
@@ -714,7 +715,7 @@ __device__ __forceinline__ u32x4 code_pairs(uint32_t w)
 }
 
 // x[T][r]: the score, short of `factor`, of slot 8 g + 4 T + r of the record for the lane's column.
-template <int NB, int NQ, bool FINE>
+template <int NB, int NQ>
 __device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Queries<NB, NQ> &q, const f32x4 &zero, f32x4 (&x)[2])
 {
     f32x4 part[2][NB];
@@ -723,7 +724,7 @@ __device__ __forceinline__ void record_scores(const KeyPart<NB> &k, const Querie
         for (int i = 0; i < NB / 2; ++i) lo[i] = k.lows[T][i];
         x[T] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, lo), q.sums, zero, 0, 0, 0);
         for (int b = 0; b < NB; ++b) {
-            const f16x8 c = __builtin_bit_cast(f16x8, code_pairs<FINE>(k.codes[T][b]));
+            const f16x8 c = __builtin_bit_cast(f16x8, code_pairs<true>(k.codes[T][b]));
             for (int p = 0; p < NQ; ++p) part[T][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, q.q[b][p], p ? part[T][b] : zero, 0, 0, 0);
         }
     }
@@ -940,7 +941,7 @@ __device__ __forceinline__ void values_by_numbers(const uint8_t *at, const uint8
 
 // One record.  A new reference exponent costs a multiplication of everything gathered, so it is taken only where a weight
 // would exceed 2^8 (32-bit sums have room for that); a lane looks at its own eight slots alone, and lanes exchange only then.
-template <int NB, int TY, bool FINE>
+template <int NB, int TY>
 __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, query_parts<TY>()> &q, int lane, int slot0, int length, bool masked,
                                               const f32x4 &zero, const Under &under, Gathered<NB> &s)
 {
@@ -949,7 +950,7 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
     {
         KeyPart<NB> k;
         take_keys<NB>(at, lane, k);
-        record_scores<NB, NQ, FINE>(k, q, zero, x);
+        record_scores<NB, NQ>(k, q, zero, x);
     }
     // Values for float16?  The lanes look at the blocks together, and leave the lowest numbers as float16 behind the record.
     bool numbers = false;
@@ -1019,7 +1020,7 @@ __device__ __forceinline__ void attend_record(uint8_t *at, const Queries<NB, que
     }
 }
 
-template <int NB, int TY, bool FINE>
+template <int NB, int TY>
 __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) void k_cache_attend(AttendArgs a)
 {
     constexpr int NQ = query_parts<TY>(), D = 32 * NB;
@@ -1052,7 +1053,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
 
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     Queries<NB, NQ> q;
-    load_queries<NB, TY, FINE ? kFine : kLow>(a, h, first, count, slot0, length, tile * kColumns + n, g, q);
+    load_queries<NB, TY, kFine>(a, h, first, count, slot0, length, tile * kColumns + n, g, q);
     Gathered<NB> acc;
     for (int i = 0; i < NB / 2; ++i)
         for (int p = 0; p < 4; ++p) acc.o[i][p] = f32x4{0, 0, 0, 0};
@@ -1073,7 +1074,7 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
         if (rec) lay_record<NB>(stage, lane, raw);
         if (next_rec) load_record<NB>(next_rec, lane, raw);
         if (rec) {
-            attend_record<NB, TY, FINE>(stage, q, lane, it * kRecordSlots + 8 * g, length,
+            attend_record<NB, TY>(stage, q, lane, it * kRecordSlots + 8 * g, length,
                                         it * kRecordSlots < all_from || (it + 1) * kRecordSlots > all_to, zero, under, acc);
         }
         it = next;
@@ -1632,7 +1633,7 @@ __global__ __launch_bounds__(256, NB == 8 || TY == kF32 ? 1 : 3) void k_cache_we
                 KeyPart<NB> keys;
                 take_keys<NB, 512, 576>(s_mem[wave][k], lane, keys);
                 f32x4 x[2];
-                record_scores<NB, NQ, true>(keys, q, f32x4{0, 0, 0, 0}, x);
+                record_scores<NB, NQ>(keys, q, f32x4{0, 0, 0, 0}, x);
                 const int from_slot = (it0 + k) * kRecordSlots + 8 * g;
                 for (int i = 0; i < 8; ++i) {
                     // (between 0 and 1: an output modifier of the power's instruction, which makes a NaN a 0)
@@ -1885,7 +1886,6 @@ static hipError_t attend_of(const AttendArgs &a, hipStream_t s)
     const uint32_t tiles = (uint32_t)a.c.n_seqs * (uint32_t)a.c.kv_heads * (uint32_t)a.tiles;
     hipError_t e = hipSuccess;
     if (tiles) {
-        // where weights are wanted the sums have to be those of the scores that they are taken from
         const dim3 grid(tiles * (uint32_t)a.splits);
         if constexpr (TY != kF32) {
             if (a.wide_tiles) {
@@ -1897,8 +1897,7 @@ static hipError_t attend_of(const AttendArgs &a, hipStream_t s)
                 if (e != hipSuccess) return e;
             }
         }
-        if (TY == kF32 || a.weights) hipLaunchKernelGGL((k_cache_attend<NB, TY, true>), grid, dim3(256), 0, s, a);
-        else if constexpr (TY != kF32) hipLaunchKernelGGL((k_cache_attend<NB, TY, false>), grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_cache_attend<NB, TY>), grid, dim3(256), 0, s, a);
         e = hipGetLastError();
         if (e == hipSuccess && a.splits > 1) {
             hipLaunchKernelGGL((k_cache_join<NB, TY>), dim3(tiles * (uint32_t)a.columns), dim3(256), 0, s, a);
