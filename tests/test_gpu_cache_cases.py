@@ -1,9 +1,11 @@
 """Further cases of the 4-bit cache on the GPU."""
+import numpy as np
 import pytest
+import torch
 
 from cache_cases import (FAR, FAR_QUERIES, check_lse_without_and_with_weights, check_rows_left_out, check_store_exact, check_weights_of_large_scores,
                          close_keys, close_queries, hard_blocks)
-from cache_world import check_attend
+from cache_world import Batch, check_attend, close
 from test_emu_cache_cases import LEFT_OUT
 from test_gpu_cache import world  # noqa: F401
 
@@ -57,3 +59,23 @@ def test_weights_of_large_scores(world, rows, group, q_scale, type_):  # noqa: F
 @pytest.mark.parametrize("d", [64, 256])
 def test_lse_without_and_with_weights(world, d, type_):  # noqa: F811
     check_lse_without_and_with_weights(world, type_, d)
+
+
+def test_many_long_sequences(world):  # noqa: F811
+    """So many that a workgroup for each would take more than 128 records: their parts are others than those of a sequence alone, what they give is
+    the same but for roundings."""
+    n, heads, d, page = 64, 8, 64, 64
+    lengths = [4200 - 61 * (i % 7) * (i % 9) for i in range(n)]
+    b = Batch(world, lengths, [1] * n, heads, d, page, seed=5)
+    b.fill()
+    assert world.cache.lib() and b.c.scratch_bytes(n, heads, n, b.table.shape[1], torch.bfloat16, max_rows=1, max_length=4200, lse=True) == n * heads * 16 * 2 * (d + 2) * 4
+    q = world.put(b.rng.standard_normal((n, heads, d)).astype(np.float32), torch.bfloat16)
+    out, lse = world.full((n, heads, d), 0.0, torch.bfloat16), world.full((n, heads), 0.0, torch.float32)
+    b.c.attend(q, out, b.d_table, b.d_lengths, b.d_starts, max_rows=1, max_length=4200, lse=lse)
+    one, one_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    for s in range(n):
+        b.c.attend(q[s:s + 1], one[s:s + 1], b.d_table[s:s + 1], b.d_lengths[s:s + 1], b.d_starts[:2], lse=one_lse[s:s + 1])
+    # (the same scores in the same waves' arithmetic: sums of 4200 terms, then roundings of out)
+    close(world.get(lse), world.get(one_lse), np.full((n, heads), 2 * 4200 * 2.0 ** -24), "lse")
+    got, want = world.get(out), world.get(one)
+    close(got, want, np.full(got.shape, 2 * 2.0 ** -8 * np.abs(want).max()), "out")

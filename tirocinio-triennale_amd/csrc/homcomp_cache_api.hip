@@ -119,14 +119,20 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
         p->wide_tiles = (p->tiles + p->tiles_in_wide - 1) / p->tiles_in_wide;
     }
     const int64_t groups = p->wide_tiles ? (int64_t)c->n_seqs * c->kv_heads * p->wide_tiles : units;   // workgroups without parts
-    // eight workgroups for every compute unit, so that sequences of different lengths even out (a single one has nothing to even out: the two
-    // that a unit holds at once), but eight records at least for every wave (and two where there is little in all).
-    // 64 sequences of up to 8192 slots, 8 heads: 95 us with eight, 98 with four, 102 with two; one of 131072: 49 with eight or four, 43 with two.
-    int64_t splits = groups ? ((p->wide_tiles || c->n_seqs == 1 ? 2 : 8) * kComputeUnits + groups - 1) / groups : 1;
-    const int64_t least = groups * records >= 64 * kComputeUnits ? 8 : 2;
-    const int64_t fine = (records + least * hc::kAttendWaves - 1) / (least * hc::kAttendWaves);
+    // Two workgroups for every compute unit, which is what one holds at once, as far as that leaves a wave two records (a short sequence: 1 x 4000 slots takes
+    // 11 us, with eight a wave 17).  Parts of more than 128 records then, of many long sequences, are cut to 64: where lengths differ, units
+    // would be idle behind the short ones.  8 heads of 128 values, four columns, us:
+    //                          1 x 131072   2 x 131072   4 x 65536   16 x 16384*   64 x 4096*   128 x 4096   32 x 16384*   64 x 8192*   64 x 8192
+    //   two a unit, cut to 64      45           70          69           61            51           126           84          107          140
+    //   two a unit                 45           69          69           61            51           127          108          105          124
+    //   four                       51           75          75           57            57           129           89          112          134
+    //   eight                      53           87          83           63            56           145           84          107          141
+    // (* lengths from a tenth to all of it.)
+    int64_t splits = groups ? (2 * kComputeUnits + groups - 1) / groups : 1;
+    const int64_t fine = (records + 2 * hc::kAttendWaves - 1) / (2 * hc::kAttendWaves);
     if (splits > fine) splits = fine;
     int64_t each = (records + splits - 1) / splits;
+    if (!p->wide_tiles && each > 128) each = (records + records / 64 - 1) / (records / 64);
     each = (each + hc::kAttendWaves - 1) / hc::kAttendWaves * hc::kAttendWaves;
     p->split_records = (int)each;
     p->splits = (int)((records + each - 1) / each);
