@@ -79,3 +79,27 @@ def test_many_long_sequences(world):  # noqa: F811
     close(world.get(lse), world.get(one_lse), np.full((n, heads), 2 * 4200 * 2.0 ** -24), "lse")
     got, want = world.get(out), world.get(one)
     close(got, want, np.full(got.shape, 2 * 2.0 ** -8 * np.abs(want).max()), "out")
+
+
+def test_selection_near_2_to_31_slots(world):  # noqa: F811
+    """The longest sequence that a table can hold: weights counted over it, then selected from its far end as from its front."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    most = (1 << 31) - 96
+    pages = world.cache.new_pages(2, 1, 64, 32)
+    c = world.cache.Cache(pages, 1, 64, 32)
+    table = torch.full((1, most // 32), -1, dtype=torch.int32, device="cuda")      # (no page: nothing to see, zeros to move)
+    lengths, starts = world.put(np.array([most], np.int32)), world.put(np.array([0, 1], np.int32))
+    weights = torch.full((1, 1, most), 33.0, device="cuda")
+    q, out, lse = world.full((1, 1, 64), 1.0, torch.bfloat16), world.full((1, 1, 64), 7.0, torch.bfloat16), world.full((1, 1), 7.0, torch.float32)
+    c.attend(q, out, table, lengths, starts, lse=lse, weights=weights)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    assert not weights[0, 0, :1000].any() and not weights[0, 0, -100000:].any() and float(weights.sum()) == 0.0
+    far = [5, 16383, 16384, 1 << 30, most - 16385, most - 96, most - 4]
+    for i, slot in enumerate(far):
+        weights[0, 0, slot] = 1.0 + i
+    to_lengths = world.full((1,), 0, torch.int32)
+    to_weights, kept = c.evict(weights, table, lengths, 12, world.full((1, 1), 1, torch.int32), to_lengths, first=2, recent=2)
+    want = sorted([0, 1, 2] + far + [most - 2, most - 1])      # (one more place than weights: the first of the zeros)
+    assert to_lengths.tolist() == [12] and kept[0, 0].tolist() == want
+    assert to_weights[0, 0].tolist() == [0.0, 0.0, 0.0] + [1.0 + i for i in range(7)] + [0.0, 0.0]
