@@ -3,7 +3,7 @@ import pytest
 
 from cache_cases import (FAR, FAR_QUERIES, check_lse_without_and_with_weights, check_rows_left_out, check_store_exact, check_weights_of_large_scores,
                          close_keys, close_queries, hard_blocks)
-from cache_world import check_attend
+from cache_world import check_attend, check_evict, check_store
 from test_emu_cache import _release, world  # noqa: F401
 
 # sequences' rows, max_rows, rows the arrays hold
@@ -58,3 +58,13 @@ def test_weights_of_large_scores(world, rows, group, q_scale, type_):  # noqa: F
 @pytest.mark.parametrize("d", [64, 256])
 def test_lse_without_and_with_weights(world, d, type_):  # noqa: F811
     check_lse_without_and_with_weights(world, type_, d)
+
+
+@pytest.mark.parametrize("n", [65, 130])
+def test_many_sequences(world, n):  # noqa: F811
+    """More than a wave looks at together when it finds its rows' sequence; some hold nothing, some get nothing."""
+    lengths = [(7 * i + i // 5) % 4 for i in range(n)]
+    rows = [min(x, (3 * i) % 3) for i, x in enumerate(lengths)]
+    check_store(world, lengths, rows, 1, 64, 32, "bf16", padding=1)
+    check_attend(world, lengths, rows, 1, 2, 64, 32, "bf16", weights=True)
+    check_evict(world, lengths, 1, 64, 32, 2, 1, 0)

@@ -5,7 +5,7 @@ import torch
 
 from cache_cases import (FAR, FAR_QUERIES, check_lse_without_and_with_weights, check_rows_left_out, check_store_exact, check_weights_of_large_scores,
                          close_keys, close_queries, hard_blocks)
-from cache_world import Batch, check_attend, close
+from cache_world import Batch, check_attend, check_evict, check_store, close
 from test_emu_cache_cases import LEFT_OUT
 from test_gpu_cache import world  # noqa: F401
 
@@ -103,3 +103,50 @@ def test_selection_near_2_to_31_slots(world):  # noqa: F811
     want = sorted([0, 1, 2] + far + [most - 2, most - 1])      # (one more place than weights: the first of the zeros)
     assert to_lengths.tolist() == [12] and kept[0, 0].tolist() == want
     assert to_weights[0, 0].tolist() == [0.0, 0.0, 0.0] + [1.0 + i for i in range(7)] + [0.0, 0.0]
+
+
+@pytest.mark.parametrize("n", [65, 129, 1500])
+def test_many_sequences(world, n):  # noqa: F811
+    """More than a wave looks at together when it finds its rows' sequence; some hold nothing, some get nothing."""
+    lengths = [(7 * i + i // 5) % 4 for i in range(n)]
+    rows = [min(x, (3 * i) % 3) for i, x in enumerate(lengths)]
+    check_store(world, lengths, rows, 1, 64, 32, "bf16", padding=1)
+    check_attend(world, lengths, rows, 1, 2, 64, 32, "bf16", weights=True)
+    check_evict(world, lengths, 1, 64, 32, 2, 1, 0)
+
+
+def test_most_sequences(world):  # noqa: F811
+    """65535 sequences of a row each: what is stored is loaded again, and a single slot's attention is its value."""
+    n = 65535
+    pages = world.cache.new_pages(n, 1, 64, 32)
+    c = world.cache.Cache(pages, 1, 64, 32)
+    table = torch.randperm(n, device="cuda").to(torch.int32)[:, None].contiguous()
+    lengths, starts = torch.ones(n, dtype=torch.int32, device="cuda"), torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    k = (torch.randint(0, 16, (n, 1, 64), device="cuda") * 0.5).bfloat16()
+    v = (torch.randint(0, 16, (n, 1, 64), device="cuda") - 7.0).bfloat16()
+    k[:, :, ::32], k[:, :, 1::32], v[:, :, ::32], v[:, :, 1::32] = 0, 7.5, -7, 8       # (steps of 1/2 and 1: held exactly)
+    c.store(k, v, table, lengths, starts)
+    back = torch.zeros_like(k), torch.zeros_like(v)
+    c.load(*back, table, lengths, starts)
+    assert torch.equal(back[0], k) and torch.equal(back[1], v)
+    out = torch.zeros_like(v)
+    c.attend(k, out, table, lengths, starts, max_rows=1, max_length=1)
+    assert torch.equal(out, v)
+    to_lengths = torch.zeros(n, dtype=torch.int32, device="cuda")
+    more = torch.cat([pages, torch.empty_like(pages)])
+    c = world.cache.Cache(more, 1, 64, 32)
+    to = table + n
+    weights, kept = c.evict(torch.rand(n, 1, 32, device="cuda"), table, lengths, 1, to, to_lengths)
+    assert (to_lengths == 1).all() and not kept.any()
+    c.load(*back, to, to_lengths, starts)
+    assert torch.equal(back[0], k) and torch.equal(back[1], v)
+
+
+@pytest.mark.parametrize("type_,kw", [("bf16", dict(weights=True)), ("f32", dict(edit=FAR[1])), ("f16", dict(window=15000))])
+def test_many_parts(world, type_, kw):  # noqa: F811
+    """One long sequence, whose parts are more than those that join them at a time."""
+    check_attend(world, [20011], [1], 1, 3, 64, 64, type_, **kw)
+
+
+def test_many_parts_of_many_columns(world):  # noqa: F811
+    check_attend(world, [9001], [9], 1, 4, 64, 64, "bf16", window=6000)
