@@ -43,6 +43,8 @@
  *     Sequences may have pages in common; rows that one call writes must have slots of their own.
  *   - Rows of numbers that a call writes (of out, or of the arrays that a load fills) share no memory, with one another or with what it reads.
  *   - A call of more workgroups than a launch can have (2^24 - 1 of 256 threads) is refused.
+ *   - A row in front of a sequence's first slot (more rows than slots) has none: it is not stored, a load leaves it as it was, and it sees what its
+ *     place says (nothing where `causal`).
  */
 #ifndef HOMCOMP_CACHE_H
 #define HOMCOMP_CACHE_H
@@ -84,11 +86,12 @@ int homcomp_cache_load(const homcomp_cache *cache, void *d_k, void *d_v, int typ
 /* Attention over the cache.  Row i of the n rows of a sequence that holds L slots is at slot a = L - n + i.  It sees the slots j < L,
  * with `causal` those j <= a, with a window w > 0 those j > a - w.  With S_j = scale * <q, k_j>:
  *   lse = log sum_j exp S_j      out = sum_j exp(S_j - lse) v_j
- * A row that sees no slot gets out = 0 and lse = -infinity.  Query head g reads the keys and values of head
+ * A row that sees no slot gets out = 0 and lse = -infinity.  Scores have to stay below 2^127 in size.  Query head g reads the keys and values of head
  * g / (q_heads / kv_heads).
  * d_weights (optional): weights[s][h][j] = prior[s][h][j] + the sum of exp(S_j - lse) over the sequence's rows and the query heads of
  * head h, for the slots j < L; what lies behind is left as it was.  d_prior NULL: 0; d_prior may be d_weights.  The sum is
- * taken in a fixed order: the same inputs give the same bits. */
+ * taken in a fixed order: the same inputs give the same bits.  A weight is exp(S_j - lse) with lse in 32 bits, at most 1: it loses digits where scores
+ * exceed 2^16. */
 typedef struct homcomp_attention {
     const void *d_q;          /* row r, query head g at element r * q_row_stride + g * q_head_stride */
     size_t q_row_stride, q_head_stride;
@@ -102,7 +105,7 @@ typedef struct homcomp_attention {
     size_t max_length;        /* no sequence holds more slots than this (a longer one is cut to its first max_length) */
     float scale;              /* finite */
     int causal;
-    size_t window;            /* 0: none */
+    size_t window;            /* 0: none.  Slots are counted, not positions: of evicted sequences it is that many of the slots left */
     float *d_lse;             /* [n_rows][q_heads], optional; memory of its own */
     const float *d_prior;     /* [n_seqs][kv_heads][weight_stride], optional */
     float *d_weights;         /* the same, optional */

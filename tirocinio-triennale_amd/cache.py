@@ -103,9 +103,9 @@ def _share_memory(rows, row, heads, head, d):
 def _meet(offset, rows, row, heads, head, d):
     """Whether the runs of two such arrays, the second `offset` elements behind the first, have an element in common."""
     offset = abs(offset)
-    row, head = row if rows > 1 else 0, head if heads > 1 else 0
     if offset >= (rows - 1) * row + (heads - 1) * head + d:
         return False
+    row, head = row if rows > 1 else 0, head if heads > 1 else 0
     for j in range(1 - heads, heads):     # offset + j * head against the rows next to there, of either sign
         at = offset + j * head
         i = at // row if row else 0
@@ -181,7 +181,8 @@ class Cache:
 
     def _own_memory(self, name, t, row, head):
         """Written tensors: no row or head of which shares another's memory."""
-        if t.numel() and _share_memory(t.shape[0], row, t.shape[1], head, self.head_dim):
+        heads, d = t.shape[1], self.head_dim
+        if (head < d or row < (heads - 1) * head + d) and t.numel() and _share_memory(t.shape[0], row, heads, head, d):   # (seldom looked at)
             raise ValueError(f"{name}: rows and heads of its own memory")
 
     def _whole(self, name, t, shape, dtype):
@@ -193,13 +194,13 @@ class Cache:
         row, head = self._numbers("k", k, self.kv_heads)
         if self._numbers("v", v, self.kv_heads) != (row, head) or k.dtype is not v.dtype or k.shape != v.shape:
             raise ValueError("k and v: of one type, shape and layout")
+        at_k, at_v, rows, type_ = k.data_ptr(), v.data_ptr(), k.shape[0], self._types[k.dtype]
         if written:
             self._own_memory("k and v", k, row, head)
-            if k.numel() and _meet((v.data_ptr() - k.data_ptr()) // k.element_size(), k.shape[0], row, k.shape[1], head, self.head_dim):
+            if rows and _meet((at_v - at_k) // (4 if type_ == F32 else 2), rows, row, self.kv_heads, head, self.head_dim):
                 raise ValueError("k and v: each of its own memory")
         args, n, _ = self._args(table, lengths)
-        self._call(name, what, args, k.data_ptr(), v.data_ptr(), self._types[k.dtype], row, head, self._starts(starts, n), k.shape[0],
-                   _stream_of(self._device, stream))
+        self._call(name, what, args, at_k, at_v, type_, row, head, self._starts(starts, n), rows, _stream_of(self._device, stream))
 
     # -- the operators ----------------------------------------------------------------------
     def store(self, k, v, table, lengths, starts, stream=None) -> None:
@@ -216,7 +217,7 @@ class Cache:
         """Attention of the rows of q ([rows, heads, head_dim], heads a multiple of kv_heads) over the slots their sequences hold.
 
         scale       of the scores, default head_dim ** -0.5
-        window      a row sees at most that many slots back, itself among them (0: all)
+        window      a row sees at most that many slots back, itself among them (0: all); after an eviction: of the slots left
         max_rows    no sequence has more rows (default: the rows of q), max_length: holds more slots (default: what the table can hold);
                     tighter numbers than the defaults make the launch smaller
         lse         float32 [rows, heads]: the log of the sum of the exponentials

@@ -321,8 +321,10 @@ __device__ __forceinline__ void wave_lds_order()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// What bounds it is quantising, 1500 vector instructions for sixteen slots of 128 values: 123 thousand slots and heads take 29 us, 2.8 TB/s of rows
-// and records.  (36 with neighbours exchanged through LDS and borders looked at value by value.)
+// 123 thousand slots and heads of 128 values take 30 us, 2.7 TB/s of rows and records.  Quantising, 1590 vector instructions for sixteen slots, keeps the
+// vector units busy for 55 % of it; the rest is that 1942 workgroups are one and a half times what the chip holds at once, and that a
+// wave loads nothing ahead.  (36 us with neighbours exchanged through LDS and borders looked at value by value; 29 before blocks whose
+// numbers lie far apart were decided exactly, which costs registers.)
 // Keys: four lanes to a slot, a lane's eight values of every block.  Values' codes of a slot lie two bytes at a time among those of seven others: the
 // wave gathers eight slots' words in LDS and writes them whole, except where not all eight are its own.
 template <int NB, int TY>
@@ -501,14 +503,14 @@ __global__ __launch_bounds__(256) void k_cache_load(CacheArgs c, RowsArgs a, uin
 //            parts where q is 32 bits wide.  The lo part is one more product over (block, part of the sums of q).
 //   values   O[value, column] = sum_slots c[slot, value] (p s_b)[slot, column] + (sum_slots lo_b p)
 //            p s_b is rounded to bfloat16 (two or three parts for outputs of 16 and 32 bits' precision); p carries 2^64 so that
-//            products with codes of 2^-133 stay normal numbers.  For 16-bit outputs a record whose values all fit float16 is multiplied as
+//            products with codes of 2^-133 stay normal numbers (see there for lo of 2^40 and more).  For 16-bit outputs a record whose values all fit float16 is multiplied as
 //            float16 numbers lo + s c instead: a third of the vector instructions.
 // A wave's two products of 16 slots each take the slots so that what lane group g gets as scores (rows 4 g + r of both) is
 // exactly what it owes the values' product as operand (slots 8 g .. 8 g + 7): nothing is exchanged between lanes.
 //
-// What bounds it is reading the records.  64 sequences of up to 8192 slots, 8 heads of 128 values, four columns each: 327 MB in 83 us, 3.9 TB/s, vector
-// instructions busy for 40 % of it (330 for a record); joining the parts adds 6 us.  One sequence of 131072
-// slots: 168 MB in 34 us, 4.9 TB/s, what a copy of the same bytes reaches.  Values as codes: 106 and 47 us.  Records through LDS
+// What bounds it is reading the records.  64 sequences of up to 8192 slots, 8 heads of 128 values, four columns each: 327 MB in 85 us, 3.8 TB/s, vector
+// instructions busy for 42 % of it (355 for a record); joining the parts adds 6 us.  One sequence of 131072
+// slots: 168 MB in 35 us, 4.8 TB/s, nearly what a copy of the same bytes reaches.  Values as codes: 106 and 47 us.  Records through LDS
 // one ahead, from where operands are taken: without it (operands loaded from memory in their order) 236 us for the batch.
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -INFINITY;
@@ -1130,16 +1132,17 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
 //
 // With more columns than one tile the records are unpacked once for all of them.  A workgroup of W waves takes 16 CT W columns; all threads
 // together unpack records into LDS, ahead of the products, as float16 numbers: keys in two parts (22 bits: scores are exponents, and lse
-// is a 32-bit result), values in one.  That rounding, and the one of p to float16 (in two parts for float16
+// is a 32-bit result; where the second part is below the normal range it still holds the places of s, which are 2^-23 and more), values in one.  That rounding, and the one of p to float16 (in two parts for float16
 // results), need numbers within float16's range.  A record with a NaN, or with blocks too large or too small for it, is not for this kernel:
 // the workgroup notes so, and k_cache_attend does its columns afterwards.
 //
 // Vector and matrix instructions about balance: for a record and 16 columns 8 multiply-adds, 8 exponentials (four times the cost
-// of others) and 25 more against 24 products of 16 cycles.  (With whole codes as keys, their scores scaled in 32 bits as above, it was 64 more
+// of others) and 25 more against 24 products of 16 cycles; a wave's share of the unpacking, which all 32 workgroups of a sequence and head do again,
+// and of finding records and keeping step is about 150 for its two tiles.  (With whole codes as keys, their scores scaled in 32 bits as above, it was 64 more
 // vector instructions for 8 products less, and 1410 us when this took 1190.)
 //
-// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1060 us, 570 TFLOP/s of the two products (603 GFLOP). The matrix unit
-// is busy 34 % of it (a third of that with the keys' second parts), vector instructions 48 %, LDS 24 %; two waves for each SIMD, which
+// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1050 us, 574 TFLOP/s of the two products (603 GFLOP), in a row of calls; the
+// first ones after other work, at a lower clock, take 1190.  The matrix unit is busy 34 % of it (a third of that with the keys' second parts), vector instructions 48 %, LDS 24 %; two waves for each SIMD, which
 // a barrier for every two records keeps in step, do not put them beside each other fully.  Keys in one part: a fifth less, but lse off by 1e-4.
 template <int NB>
 struct WideRecord {
@@ -1512,8 +1515,9 @@ __global__ __launch_bounds__(256) void k_cache_join(AttendArgs a)
 // The attention each slot received.  A wave holds two records' keys in LDS (the next two on their way) and goes over all columns of their
 // sequence and head, computing the scores again, and adds in the columns' order.  (Keeping the scores of the attention kernel instead
 // would write and read 4 bytes for every column and slot: with four columns 32 bytes a slot, with eight 64, against the 80 of the keys of
-// 128 values.)  Between reading a cache's keys and computing: 25000 records and four columns take 28 us, 34 where a workgroup ends after
-// eight records (its start - positions, page, queries - costs as much as four), 40000 columns of 2048 rows on 5000 records 2 ms.
+// 128 values.)  Between reading a cache's keys and computing: 25000 records and four columns take 30 us, six more where a workgroup ends after
+// eight records (its start - positions, page, queries - costs as much as four).  For many rows it is far from its products' time: 2 x 2048 rows of
+// 32 heads on 10007 slots take 2.0 ms, as codes are unpacked, and scores scaled block by block, again for every 16 columns.
 // Four or eight records held: the same for few columns, 8 and 20 % slower for many (fewer waves fit).
 constexpr int kHeldRecords = 2, kWeightsPerUnit = 2;   // workgroups for a compute unit, where there are batches for more
 
@@ -1691,7 +1695,8 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t *sums, 
 // A workgroup per sequence and head.  A thread holds sixteen neighbouring weights, so that ranks need one prefix sum over the threads; sequences
 // of up to 16384 slots are read once, longer ones once for each of the passes.  The key of the last weight to stay is found 11,
 // 11 and 10 bits at a time from the top: counts in LDS, then a prefix sum from the largest bin down.
-// Bound by the passes' barriers and instructions, not by memory: 128 heads of up to 16384 slots take 16 us, 8 of 1100 slots 10.
+// Bound by the passes' barriers and instructions, not by memory: 128 heads of up to 16384 slots take 16 us, 8 of 1100 slots 10; ten of 31995,
+// whose weights are read once a pass, 40.
 __global__ __launch_bounds__(kSelectThreads) void k_cache_select(EvictArgs a)
 {
     __shared__ uint32_t s_bins[kSelectBins];
