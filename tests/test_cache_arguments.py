@@ -95,3 +95,25 @@ def test_one_row_or_none(call):
             call.attend(q=torch.zeros(n, 4, 64), out=torch.zeros(n, 4, 64).as_strided((n, 4, 64), (3, 64, 1)))
     with pytest.raises(ValueError, match="GPU"):
         call.store(k=rows_of(MEMORY, (0, 64, 1), 2), v=rows_of(MEMORY, (0, 64, 1), 2))      # (read alone)
+
+
+def test_scratch_does_not_grow_with_the_lengths(cache):  # noqa: F811
+    """Parts are cut for workgroups to be enough, at most eight a compute unit where there are not as many anyway: memory for them has a bound."""
+    rng = random.Random(5)
+    for _ in range(3000):
+        heads, group, d = rng.choice([1, 2, 8, 32]), rng.choice([1, 4, 16, 40]), rng.choice([64, 128, 256])
+        n, rows = rng.choice([1, 2, 7, 64, 300]), rng.choice([0, 1, 1, 5, 64, 3000, 20000])
+        length = rng.choice([100, 5000, 131072, 1 << 20, 1 << 24])
+        if n * rows * heads * group >= 1 << 31:
+            continue
+        type_ = rng.choice([torch.bfloat16, torch.float32])
+        c = cache.Cache(torch.zeros(0, dtype=torch.uint8), heads, d, 64)
+        need = c.scratch_bytes(n * rows, heads * group, n, -(-length // 64), type_, max_rows=rows, lse=True)
+        tiles = -(-rows * group // 16)
+        units = n * heads * tiles
+        wide = type_ == torch.bfloat16 and tiles > 1
+        # (a wide workgroup takes up to sixteen tiles)
+        most = (2048 + units) * (16 if wide else 1) * 16 * (d + 2) * 4
+        assert need <= most, (heads, group, d, n, rows, length, type_, need, most)
+        if not wide and units >= 2048:
+            assert need == 0, (heads, group, d, n, rows, length, type_, need)

@@ -120,10 +120,11 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
     }
     const int64_t groups = p->wide_tiles ? (int64_t)c->n_seqs * c->kv_heads * p->wide_tiles : units;   // workgroups without parts
     // Two workgroups for every compute unit, which is what one holds at once, as far as that leaves a wave two records (a short sequence: 1 x 4000 slots takes
-    // 11 us, with eight a wave 17).  Parts of more than 128 records then, of many long sequences, are cut to 64: where lengths differ, units
-    // would be idle behind the short ones.  8 heads of 128 values, four columns, us:
+    // 11 us, with eight a wave 17).  Where that makes parts of more than 128 records of several sequences: up to eight a unit, of 64 records at least, as
+    // units would be idle behind the shorter ones (a single sequence has none: 1 x 524288 takes 125 us whole, 151 cut).
+    // 8 heads of 128 values, four columns, us:
     //                          1 x 131072   2 x 131072   4 x 65536   16 x 16384*   64 x 4096*   128 x 4096   32 x 16384*   64 x 8192*   64 x 8192
-    //   two a unit, cut to 64      45           70          69           61            51           126           84          107          140
+    //   two a unit, or cut         45           70          69           61            51           126           84          107          140
     //   two a unit                 45           69          69           61            51           127          108          105          124
     //   four                       51           75          75           57            57           129           89          112          134
     //   eight                      53           87          83           63            56           145           84          107          141
@@ -132,7 +133,11 @@ int plan_attention(const homcomp_cache *c, const homcomp_attention *t, int nb, i
     const int64_t fine = (records + 2 * hc::kAttendWaves - 1) / (2 * hc::kAttendWaves);
     if (splits > fine) splits = fine;
     int64_t each = (records + splits - 1) / splits;
-    if (!p->wide_tiles && each > 128) each = (records + records / 64 - 1) / (records / 64);
+    if (!p->wide_tiles && c->n_seqs > 1 && groups > 0 && each > 128) {
+        int64_t more = (8 * kComputeUnits + groups - 1) / groups;
+        if (more > records / 64) more = records / 64;
+        each = (records + more - 1) / more;
+    }
     each = (each + hc::kAttendWaves - 1) / hc::kAttendWaves * hc::kAttendWaves;
     p->split_records = (int)each;
     p->splits = (int)((records + each - 1) / each);
