@@ -503,8 +503,8 @@ __global__ __launch_bounds__(256) void k_cache_load(CacheArgs c, RowsArgs a, uin
 //            parts where q is 32 bits wide.  The lo part is one more product over (block, part of the sums of q).
 //   values   O[value, column] = sum_slots c[slot, value] (p s_b)[slot, column] + (sum_slots lo_b p)
 //            p s_b is rounded to bfloat16 (two or three parts for outputs of 16 and 32 bits' precision); p carries 2^64 so that
-//            products with codes of 2^-133 stay normal numbers (see there for lo of 2^40 and more).  For 16-bit outputs a record whose values all fit float16 is multiplied as
-//            float16 numbers lo + s c instead: a third of the vector instructions.
+//            products with codes of 2^-133 stay normal numbers (see there for lo of 2^40 and more).  For 16-bit outputs a record whose
+//            values all fit float16 is multiplied as float16 numbers lo + s c instead: a third of the vector instructions.
 // A wave's two products of 16 slots each take the slots so that what lane group g gets as scores (rows 4 g + r of both) is
 // exactly what it owes the values' product as operand (slots 8 g .. 8 g + 7): nothing is exchanged between lanes.
 //
@@ -1131,19 +1131,20 @@ __global__ __launch_bounds__(256, NB == 8 || (NB == 4 && TY == kF32) ? 1 : 2) vo
 // ---------------------------------------------------------------- attention of many rows
 //
 // With more columns than one tile the records are unpacked once for all of them.  A workgroup of W waves takes 16 CT W columns; all threads
-// together unpack records into LDS, ahead of the products, as float16 numbers: keys in two parts (22 bits: scores are exponents, and lse
-// is a 32-bit result; where the second part is below the normal range it still holds the places of s, which are 2^-23 and more), values in one.  That rounding, and the one of p to float16 (in two parts for float16
-// results), need numbers within float16's range.  A record with a NaN, or with blocks too large or too small for it, is not for this kernel:
-// the workgroup notes so, and k_cache_attend does its columns afterwards.
+// together unpack records into LDS, ahead of the products, as float16 numbers: values in one part, keys in two (22 bits: scores are exponents,
+// and lse is a 32-bit result; where a second part is below the normal range it still holds the places of s, which are 2^-23 and more).  That
+// rounding, and the one of p to float16 (in two parts for float16 results), need numbers within float16's range.  A record with a NaN, or with
+// blocks too large or too small for it, is not for this kernel: the workgroup notes so, and k_cache_attend does its columns afterwards.
 //
 // Vector and matrix instructions about balance: for a record and 16 columns 8 multiply-adds, 8 exponentials (four times the cost
-// of others) and 25 more against 24 products of 16 cycles; a wave's share of the unpacking, which all 32 workgroups of a sequence and head do again,
-// and of finding records and keeping step is about 150 for its two tiles.  (With whole codes as keys, their scores scaled in 32 bits as above, it was 64 more
-// vector instructions for 8 products less, and 1410 us when this took 1190.)
+// of others) and 25 more against 24 products of 16 cycles; a wave's share of the unpacking, which all 32 workgroups of a sequence and head do
+// again, of finding records and keeping step is about 150 for its two tiles.  (With whole codes as keys, their scores scaled in 32 bits as
+// above, it was 64 more vector instructions for 8 products less, and 1410 us when this took 1190.)
 //
-// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1050 us, 574 TFLOP/s of the two products (603 GFLOP), in a row of calls; the
-// first ones after other work, at a lower clock, take 1190.  The matrix unit is busy 34 % of it (a third of that with the keys' second parts), vector instructions 48 %, LDS 24 %; two waves for each SIMD, which
-// a barrier for every two records keeps in step, do not put them beside each other fully.  Keys in one part: a fifth less, but lse off by 1e-4.
+// 2 x 2048 rows of 32 heads over 10007 slots, 8 heads of 128 values, bfloat16: 1050 us, 574 TFLOP/s of the two products (603 GFLOP), in a row of
+// calls; the first ones after other work, at a lower clock, take 1190.  The matrix unit is busy 34 % of it (a third of that with the keys'
+// second parts), vector instructions 48 %, LDS 24 %; two waves for each SIMD, which a barrier for every two records keeps in step, do not
+// put them beside each other fully.  Keys in one part: a fifth less, but lse off by 1e-4.
 template <int NB>
 struct WideRecord {
     static constexpr uint32_t kRest = 2048u * NB, kValues = 4096u * NB, kBytes = 6144u * NB;   // keys from 0, their second parts
